@@ -11,7 +11,6 @@ sequence: they are its last ones, at positions seq_len - n .. seq_len - 1.
   attention of the query at position p over 0 <= t <= p (or t < seq_len, not causal) and t > p - window (window > 0):
             softmax(q . k_t / sqrt(head_dim)) . v_t
 """
-import functools
 import math
 import sys
 from pathlib import Path
@@ -253,9 +252,7 @@ def _plain_attend(s):
 
 
 # ---- the framework's calls -------------------------------------------------
-@functools.cache
 def _ext():
-    """The package, imported once as a user's program does."""
     here = str(Path(__file__).resolve().parents[1] / "lsq-lowbit-optimization_b200")
     if here not in sys.path:
         sys.path.insert(0, here)
