@@ -13,8 +13,7 @@
 //
 // Bound by instruction issue: about 600 instructions for 32 tokens of a head, a third of them the shifts and
 // logic that unpack. One sequence of 131072 tokens, 32 query heads on 8 of 128 channels, bfloat16:
-// 43 us, 3.3 TB/s; 4.65 TB/s from token to token, and 12 us for the start and the join. 64 sequences of up to 8192
-// tokens, 64 heads on 8: 96 us, 3.2 TB/s.
+// 48 us, 3.0 TB/s. 64 sequences of up to 8192 tokens, 64 heads on 8: 108 us, 2.9 TB/s.
 //
 // Codes. A 32-bit word of a row is eight channels; word & 0x000f000f is the pair (0, 4),
 // >> 8 the pair (2, 6). With the sign bit flipped a nibble is n = c + 8 >= 0.
@@ -28,9 +27,11 @@
 //    scores of standard deviation 4, 1e-6 to 2e-6 with two float16 roundings in one sum.
 //  * Values: as bfloat16 bits, 0x4300 | n is 128 + n, and 136 is subtracted (exact). Here the
 //    sums run over thousands of tokens and would cancel 136 sum(p) to its last bits.
-// Weights times the value's scale are rounded to bfloat16, whose range is that of the scales; for
-// float16 queries their remainder is a second bfloat16 (16 bits in all), for float32 ones there is a third
-// (24): one more product each.
+// Weights times the value's scale are bfloat16 terms, whose range is that of the scales: two, which keep 15 bits, and
+// for float32 queries three (24 bits), with a product each. The two come from two terms of the weight by three bfloat16
+// multiply-adds, since what the first product leaves is exact in bfloat16. With one term only a call takes 44.5 us in place
+// of 48.3 (131072 tokens) and 97 in place of 108 (64 sequences), but its rounding adds as much to the error as that of a bfloat16
+// output: 2.3e-3 against 1.7e-3 from the formula in 64 bits.
 #pragma once
 
 #include "kv_cache.cuh"
@@ -151,16 +152,16 @@ __device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* m
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(0), "r"(row), "r"(head), "r"(page)
       : "memory");
 }
-template <int kWords>
+template <int kWords, int kAlign>
 __device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&r)[kWords]) {
-  if constexpr (kWords % 4 == 0) {
+  if constexpr (kWords % 4 == 0 && kAlign % 16 == 0) {
 #pragma unroll
     for (int i = 0; i < kWords; i += 4)
       asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                    : "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3])
                    : "r"(addr + 4 * i)
                    : "memory");
-  } else if constexpr (kWords % 2 == 0) {
+  } else if constexpr (kWords % 2 == 0 && kAlign % 8 == 0) {
 #pragma unroll
     for (int i = 0; i < kWords; i += 2)
       asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r[i]), "=r"(r[i + 1]) : "r"(addr + 4 * i) : "memory");
@@ -169,6 +170,29 @@ __device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&r)[kWords]) 
     for (int i = 0; i < kWords; ++i)
       asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r[i]) : "r"(addr + 4 * i) : "memory");
   }
+}
+__device__ __forceinline__ uint32_t lds_u16(uint32_t addr) {
+  uint16_t x;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(addr) : "memory");
+  return x;
+}
+__device__ __forceinline__ void sts_u16(uint32_t addr, uint16_t x) {
+  asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(x) : "memory");
+}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t neg_bf16x2(uint32_t a) {
+  uint32_t d;
+  asm("neg.bf16x2 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
 }
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
@@ -278,6 +302,29 @@ struct AttnTile {
   }
 };
 
+// Values' scales of the token pairs 8 k + 2 t4, + 1 (k = 0 .. 3) for one group, as bfloat16 pairs. Two groups share a word of a
+// token where their number is even; where it is odd, words hold a key's and a value's.
+template <typename Tile>
+struct PairScales {
+  static constexpr int kGroups = Tile::kGroups;
+  uint32_t w[4][2];
+  __device__ __forceinline__ void load(uint32_t scales, int t4, int grp) {
+    const int e = kGroups + grp;  // its place among a token's scales
+    if (grp && e % 2) return;     // the word of the group before
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t r[1];
+        lds_words<1, 4>(scales + (8 * k + 2 * t4 + i) * Tile::kScaleBytes + e / 2 * 4, r);
+        w[k][i] = r[0];
+      }
+  }
+  __device__ __forceinline__ uint32_t get(int k, int grp) const {
+    return __byte_perm(w[k][0], w[k][1], (kGroups + grp) % 2 ? 0x7632 : 0x5410);
+  }
+};
+
 // Dynamic shared memory of a block: the warps' stages, later their results.
 template <int D, int G, int NT>
 constexpr int attn_smem_bytes() {
@@ -296,8 +343,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_sm(D, NT, sizeof(
     kv_attn_int4_kernel(const __grid_constant__ AttnParams p) {
   using Tile = AttnTile<D, G>;
   constexpr int QT = sizeof(T) == 4 ? 2 : 1;                     // float16 terms of a query
-  constexpr int PT = sizeof(T) == 4 ? 3 : std::is_same<T, __nv_bfloat16>::value ? 1 : 2;  // bfloat16 terms of a weight
+  constexpr int PT = sizeof(T) == 4 ? 3 : 2;                     // bfloat16 terms of a weight
   constexpr bool kSigned = QT > 1;  // keys' codes are made signed first
+  constexpr bool kPairs = PT == 2;  // weights take up the values' scales in pairs of tokens
   constexpr int kSegs = D / 32, kSegsGroup = G / 32, kGroups = Tile::kGroups, kStages = Tile::kStages;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ uint64_t full_bar[Tile::kRing];
@@ -526,11 +574,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_sm(D, NT, sizeof(
     const uint32_t codes = my_codes + st * 2 * Tile::kCodes;
     const int t0 = begin + (warp + j * kAttnWarps) * kTile;
 
-    // Scales of tokens g, g + 8, g + 16, g + 24: keys' groups, then values'.
-    uint32_t sc[4][kGroups];
+    // Scales of tokens g, g + 8, g + 16, g + 24: keys' groups, then values' (not for pairs).
+    const uint32_t scales = my_scales + st * Tile::kScales;
+    uint32_t sc[4][kPairs ? (kGroups + 1) / 2 : kGroups];
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      lds_words<kGroups>(my_scales + st * Tile::kScales + (g + 8 * k) * Tile::kScaleBytes, sc[k]);
+      lds_words<kPairs ? (kGroups + 1) / 2 : kGroups, Tile::kScaleBytes>(scales + (g + 8 * k) * Tile::kScaleBytes, sc[k]);
     auto scale_of = [&](int k, int e) { return e & 1 ? bf16_hi(sc[k][e >> 1]) : bf16_lo(sc[k][e >> 1]); };
 
     float s[2][NT][4];  // [16-token half][n-tile]: tokens g, g + 8 x query rows 2 t4, 2 t4 + 1
@@ -597,24 +646,26 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_sm(D, NT, sizeof(
           }
       // A hidden value's weight is 0, and its scale may be NaN or infinite: take those groups out of the products, and
       // give NaN to the rows that do see such a value.
+      auto v_scale_at = [&](int k, int grp) {
+        return scales + (g + 8 * k) * Tile::kScaleBytes + 2 * (kGroups + grp);
+      };
+      auto v_scale = [&](int k, int grp) {
+        if constexpr (kPairs) return bf16_lo(lds_u16(v_scale_at(k, grp)));
+        else return scale_of(k, kGroups + grp);
+      };
       bool nan = false;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int grp = 0; grp < kGroups; ++grp) {
-          const float vs = scale_of(k, kGroups + grp);
-          nan |= !(fabsf(vs) <= 3.4e38f);
-        }
+        for (int grp = 0; grp < kGroups; ++grp) nan |= !(fabsf(v_scale(k, grp)) <= 3.4e38f);
       if (__any_sync(0xffffffffu, nan)) {
 #pragma unroll
         for (int grp = 0; grp < kGroups; ++grp) {
           bool hit[NT][2] = {};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const int e = kGroups + grp;
-            const float vs = scale_of(k, e);
-            if (fabsf(vs) <= 3.4e38f) continue;
-            sc[k][e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
+            if (fabsf(v_scale(k, grp)) <= 3.4e38f) continue;
+            if constexpr (!kPairs) sc[k][(kGroups + grp) >> 1] &= (kGroups + grp) & 1 ? 0x0000ffffu : 0xffff0000u;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -631,6 +682,15 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_sm(D, NT, sizeof(
                   o[k][nt][r] = o[k][nt][r + 2] = __uint_as_float(0x7fc00000u);
               }
             }
+        }
+        if constexpr (kPairs) {  // four lanes have the same token
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int grp = 0; grp < kGroups; ++grp)
+              if (t4 == 0 && !(fabsf(v_scale(k, grp)) <= 3.4e38f)) sts_u16(v_scale_at(k, grp), 0);
+          __syncwarp();
         }
       }
     }
@@ -679,26 +739,57 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_sm(D, NT, sizeof(
       }
 
     // O^T += V^T (P scale)^T. Half h holds tokens 16 h .. 16 h + 15 as its 16 products.
-#pragma unroll
-    for (int grp = 0; grp < kGroups; ++grp) {
-      uint32_t pb[PT][2][NT][2];  // [term][half][n-tile][tokens 0-7, 8-15]
+    uint32_t wt[2][2][NT][2];  // pairs: terms of the weights as right operands, [term][half][n-tile][tokens 0-7, 8-15]
+    if constexpr (kPairs) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float vs = scale_of(2 * h + k, kGroups + grp);
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const float x = s[h][nt][2 * k] * vs, y = s[h][nt][2 * k + 1] * vs;
-            float rx = x, ry = y;
+          for (int k = 0; k < 2; ++k) {
+            const float x = s[h][nt][2 * k], y = s[h][nt][2 * k + 1];
+            const uint32_t w = pack_bf16(x, y);
+            wt[0][h][nt][k] = movmatrix(w);
+            wt[1][h][nt][k] = movmatrix(pack_bf16(x - bf16_lo(w), y - bf16_hi(w)));
+          }
+    }
+    PairScales<Tile> pair_scales;
 #pragma unroll
-            for (int term = 0; term < PT; ++term) {
-              const uint32_t w = pack_bf16(rx, ry);
-              pb[term][h][nt][k] = movmatrix(w);
-              rx -= bf16_lo(w), ry -= bf16_hi(w);
+    for (int grp = 0; grp < kGroups; ++grp) {
+      uint32_t pb[PT][2][NT][2];  // [term][half][n-tile][tokens 0-7, 8-15]
+      if constexpr (kPairs) {
+        pair_scales.load(scales, t4, grp);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t vs = pair_scales.get(2 * h + k, grp);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint32_t x = mul_bf16x2(wt[0][h][nt][k], vs), left = fma_bf16x2(wt[0][h][nt][k], vs, neg_bf16x2(x));
+              pb[0][h][nt][k] = x;
+              pb[1][h][nt][k] = fma_bf16x2(wt[1][h][nt][k], vs, left);
             }
           }
-        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float vs = scale_of(2 * h + k, kGroups + grp);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const float x = s[h][nt][2 * k] * vs, y = s[h][nt][2 * k + 1] * vs;
+              float rx = x, ry = y;
+#pragma unroll
+              for (int term = 0; term < PT; ++term) {
+                const uint32_t w = pack_bf16(rx, ry);
+                pb[term][h][nt][k] = movmatrix(w);
+                rx -= bf16_lo(w), ry -= bf16_hi(w);
+              }
+            }
+          }
+      }
 #pragma unroll
       for (int seg = grp * kSegsGroup; seg < (grp + 1) * kSegsGroup; ++seg) {
         uint32_t w[4];

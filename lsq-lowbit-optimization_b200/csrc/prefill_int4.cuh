@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
 #pragma unroll 1
         for (int k = g * (G / 32); k < (g + 1) * (G / 32); ++k) {
           uint32_t w[4];
-          lds_words<4>(src + AttnTile<D, G>::place(r, k), w);
+          lds_words<4, 16>(src + AttnTile<D, G>::place(r, k), w);
 #pragma unroll
           for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(dst + pre_place(r, k * 4 + q)) = unpack8(w[q], s);
         }
