@@ -304,8 +304,8 @@ W4A8_API int w4a8_kv_read_int4(const w4a8_kv_cache* cache, void* k, void* v, int
  * batch and max_q must be positive (rows 0: nothing to do). max_q and max_len bound the packed rows and tokens of a sequence. The
  * splitting of the work goes by max_len: a larger one is right too, and a
  * smaller one only slower.
- * workspace: w4a8_attention_int4_workspace bytes (0 for calls that are not
- * split), 16-byte aligned, this call's own until it has run. */
+ * workspace: w4a8_attention_int4_workspace bytes (0 for calls of few rows
+ * that are not split), 16-byte aligned, this call's own until it has run. */
 W4A8_API int w4a8_attention_int4(const w4a8_kv_cache* cache, const void* q, int64_t q_row, int64_t q_head, int q_heads,
                         int dtype, void* out, float* lse, float scale, int causal, int window, int max_q, int max_len,
                         void* workspace, size_t workspace_bytes, void* stream);

@@ -65,13 +65,17 @@ int make_plan(const w4a8_kv_cache* c, int q_heads, int dtype, int max_q, int max
   chunk = (chunk + least - 1) / least * least;
   p->chunk = int(std::min<long long>(chunk, 0x7fffffff / least * least));
   p->splits = int(std::max(1ll, (tokens + chunk - 1) / chunk));
-  if (p->tiles * p->splits > 0x7fffffff) return W4A8_ERR_UNSUPPORTED;
+  if (p->tiles * (p->n_tiles ? p->splits : std::max(p->splits, kRedoParts)) > 0x7fffffff) return W4A8_ERR_UNSUPPORTED;
   return W4A8_OK;
 }
 
-size_t workspace_of(const w4a8_kv_cache* c, int q_heads, const Plan& p) {
+// Partial results of calls that are split, then a word for each block of many rows.
+size_t parts_of(const w4a8_kv_cache* c, int q_heads, const Plan& p) {
   if (p.splits == 1) return 0;
   return size_t(c->rows) * q_heads * p.splits * (size_t(c->head_dim) + 2) * 4;
+}
+size_t workspace_of(const w4a8_kv_cache* c, int q_heads, const Plan& p) {
+  return parts_of(c, q_heads, p) + (p.n_tiles ? 0 : size_t(p.tiles) * p.splits * 4);
 }
 
 int check(const w4a8_kv_cache* c, int q_heads, int dtype, int max_q, int max_len, int window) {
@@ -114,7 +118,7 @@ extern "C" int w4a8_attention_int4(const w4a8_kv_cache* cache, const void* q, in
   Plan plan;
   rc = make_plan(cache, q_heads, dtype, max_q, max_len, window, &plan);
   if (rc != W4A8_OK) return rc;
-  const size_t need = workspace_of(cache, q_heads, plan);
+  const size_t need = workspace_of(cache, q_heads, plan), parts = parts_of(cache, q_heads, plan);
   if (need > workspace_bytes || (need && !workspace)) return W4A8_ERR_ARG;
   if (need && reinterpret_cast<uintptr_t>(workspace) % 16) return W4A8_ERR_ALIGN;
   p.q = q;
@@ -140,7 +144,8 @@ extern "C" int w4a8_attention_int4(const w4a8_kv_cache* cache, const void* q, in
   p.by_heads = fast_div(unsigned(cache->heads));
   p.chunk = plan.chunk;
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + (need ? size_t(cache->rows) * q_heads * plan.splits * cache->head_dim : 0));
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + (parts ? size_t(cache->rows) * q_heads * plan.splits * cache->head_dim : 0));
+  p.handover = plan.n_tiles ? nullptr : reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + parts);
   const unsigned grid = unsigned(plan.tiles * plan.splits);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (cache->head_dim) {

@@ -21,7 +21,8 @@
 //    without any conversion. The query is scaled to a largest magnitude near 2^14 by a power of
 //    two, its pairs (1, 5) and (3, 7) are divided by 16, and the accumulators start at
 //    -8 2^-24 sum(q): sums of a group come out signed. They are multiplied by the key's scale in
-//    32 bits. For float32 queries 8 is subtracted from n first, and the query is two terms with sums of
+//    32 bits. (The tensor cores cut products off 25 bits below the largest of a step, and count a subnormal as 2^-14
+//    there: what a channel adds to a score is off by up to 2^-15 of the largest |q| times the key's scale.) For float32 queries 8 is subtracted from n first, and the query is two terms with sums of
 //    their own: the scaled query rounded to multiples of 8, whose sums are integers below 2^24 and so exact (the
 //    tensor cores cut off what lies below the largest product of a step), and what is left. Off by 2e-7 to 3e-7 for
 //    scores of standard deviation 4, 1e-6 to 2e-6 with two float16 roundings in one sum.
@@ -63,6 +64,7 @@ struct AttnParams {
   int splits, chunk;        // blocks a sequence, tokens a block
   float* part_o;            // [rows * q_heads][splits][D]
   float2* part_ml;          // [rows * q_heads][splits]: largest score (log2), sum of weights
+  int* handover;            // many rows: for each block, whether its rows are left to kv_attn_redo_kernel
 };
 
 // Token and head of query row r of a key head, by division with by_ratio.
@@ -338,52 +340,20 @@ constexpr int attn_blocks_sm(int d, int nt, bool f32) {
   return nt == 1 && d <= 128 && !f32 ? 4 : nt == 1 && d <= 128 ? 3 : 2;
 }
 
+// Query rows [r0, r1), at most 8 NT, of a key head over the tokens [begin, end), by a block. splits > 1: partial results of
+// piece `split`. box_rows: 0, or p.box_rows with barriers that were initialised.
 template <typename T, int D, int G, int NT>
-__global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_sm(D, NT, sizeof(T) == 4))
-    kv_attn_int4_kernel(const __grid_constant__ AttnParams p) {
+__device__ __forceinline__ void attn_rows(const AttnParams& p, const KvSeq& seq, int b, int head, int r0, int r1, int begin,
+                                          int end, int split, int splits, int box_rows, uint8_t* smem, uint64_t* full_bar,
+                                          int* abort_flag) {
   using Tile = AttnTile<D, G>;
   constexpr int QT = sizeof(T) == 4 ? 2 : 1;                     // float16 terms of a query
   constexpr int PT = sizeof(T) == 4 ? 3 : 2;                     // bfloat16 terms of a weight
   constexpr bool kSigned = QT > 1;  // keys' codes are made signed first
   constexpr bool kPairs = PT == 2;  // weights take up the values' scales in pairs of tokens
   constexpr int kSegs = D / 32, kSegsGroup = G / 32, kGroups = Tile::kGroups, kStages = Tile::kStages;
-  extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ uint64_t full_bar[Tile::kRing];
-  __shared__ int abort_flag;
-  pdl_trigger();
   const KvView& v = p.view;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-
-  if (p.box_rows) {
-    if (threadIdx.x < Tile::kRing) mbar_init(&full_bar[threadIdx.x], 1);
-    if (threadIdx.x == 0) {
-      abort_flag = 0;
-      tma_prefetch_desc(&p.k_map);
-      tma_prefetch_desc(&p.v_map);
-    }
-    fence_mbarrier_init();
-    __syncthreads();
-  }
-  const BlockWork work = block_work(p, blockIdx.x);
-  const int split = work.split, row_tile = work.row_tile, head = work.head, b = work.b;
-  pdl_wait();
-  if (v.cu_q && blockIdx.x < kClearBlocks)
-    attn_clear_outside<T>(p, int(blockIdx.x), min(int(gridDim.x), kClearBlocks));
-  const KvSeq seq = kv_seq(v, b);
-  if (seq.n > p.max_q) {
-    kv_error(v);
-    if (row_tile == 0 && split == 0)
-      attn_clear_rows<T>(p, seq.row0, seq.row0 + seq.n, head * p.ratio, p.ratio);
-    return;
-  }
-  const int rows = seq.n * p.ratio, r0 = row_tile * 8 * NT;
-  if (r0 >= rows) return;
-  const int r1 = min(rows, r0 + 8 * NT);
-  int begin, end;
-  attn_range(p, seq, r0, r1, kTile, &begin, &end);
-  begin += split * p.chunk;
-  if (begin >= end && split) return;  // the join counts the splits that have tokens
-  if (split + 1 < p.splits) end = min(end, begin + p.chunk);  // the last one takes what is left
 
   const int ring = warp * kStages;
   const uint32_t my_codes = smem_u32(smem) + ring * 2 * Tile::kCodes;
@@ -421,10 +391,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_sm(D, NT, sizeof(
         if constexpr (Tile::kScalePiece == 16) cp_async_16(dst, src + k, have);
         else cp_async_ca<Tile::kScalePiece>(dst, src + k, have);
       }
-      if (p.box_rows) {
-        const bool copies = have && lane % p.box_rows == 0;
+      if (box_rows) {
+        const bool copies = have && lane % box_rows == 0;
         const unsigned boxes = __popc(__ballot_sync(0xffffffffu, copies));
-        if (lane == 0) mbar_arrive_expect_tx(&full_bar[ring + st], boxes * 2u * unsigned(p.box_rows) * Tile::kPitch);
+        if (lane == 0) mbar_arrive_expect_tx(&full_bar[ring + st], boxes * 2u * unsigned(box_rows) * Tile::kPitch);
         __syncwarp();
         if (copies) {
           const uint32_t bar = smem_u32(&full_bar[ring + st]), dst = codes + lane * Tile::kPitch;
@@ -561,8 +531,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_sm(D, NT, sizeof(
     load_tile(j + kStages - 1);
     cp_async_wait<kStages - 1>();
     const int st = j % kStages;
-    if (p.box_rows &&
-        !__all_sync(0xffffffffu, mbar_wait(&full_bar[ring + st], (j / kStages) & 1, &abort_flag))) {
+    if (box_rows &&
+        !__all_sync(0xffffffffu, mbar_wait(&full_bar[ring + st], (j / kStages) & 1, abort_flag))) {
       // A copy did not arrive: leave without any in flight.
       if (lane == 0) atomicOr(v.err, kErrTimeoutProducer);
       for (int k = j; k < min(my_tiles, j + kStages); ++k)
@@ -863,16 +833,58 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_sm(D, NT, sizeof(
     const int r = r0 + row;
     const QueryRow qr = query_row(p, r);
     const long long at = (long long)(seq.row0 + qr.token) * p.q_heads + head * p.ratio + qr.head;
-    if (p.splits > 1) {
-      float4* dst = reinterpret_cast<float4*>(p.part_o + (at * p.splits + split) * D + d);
+    if (splits > 1) {
+      float4* dst = reinterpret_cast<float4*>(p.part_o + (at * splits + split) * D + d);
       *dst = make_float4(x[0], x[1], x[2], x[3]);
-      if (d == 0) p.part_ml[at * p.splits + split] = make_float2(top, sum);
+      if (d == 0) p.part_ml[at * splits + split] = make_float2(top, sum);
     } else {
       const float inv = sum == 0.0f ? 0.0f : __frcp_rn(sum);
       store4(static_cast<T*>(p.out) + at * D + d, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
       if (d == 0 && p.lse) p.lse[at] = sum == 0.0f ? kNegInf : (top + log2f(sum)) * 0.69314718055994531f;
     }
   }
+}
+
+template <typename T, int D, int G, int NT>
+__global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_sm(D, NT, sizeof(T) == 4))
+    kv_attn_int4_kernel(const __grid_constant__ AttnParams p) {
+  using Tile = AttnTile<D, G>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ uint64_t full_bar[Tile::kRing];
+  __shared__ int abort_flag;
+  pdl_trigger();
+  const KvView& v = p.view;
+  if (p.box_rows) {
+    if (threadIdx.x < Tile::kRing) mbar_init(&full_bar[threadIdx.x], 1);
+    if (threadIdx.x == 0) {
+      abort_flag = 0;
+      tma_prefetch_desc(&p.k_map);
+      tma_prefetch_desc(&p.v_map);
+    }
+    fence_mbarrier_init();
+    __syncthreads();
+  }
+  const BlockWork work = block_work(p, blockIdx.x);
+  const int split = work.split, row_tile = work.row_tile, head = work.head, b = work.b;
+  pdl_wait();
+  if (v.cu_q && blockIdx.x < kClearBlocks)
+    attn_clear_outside<T>(p, int(blockIdx.x), min(int(gridDim.x), kClearBlocks));
+  const KvSeq seq = kv_seq(v, b);
+  if (seq.n > p.max_q) {
+    kv_error(v);
+    if (row_tile == 0 && split == 0)
+      attn_clear_rows<T>(p, seq.row0, seq.row0 + seq.n, head * p.ratio, p.ratio);
+    return;
+  }
+  const int rows = seq.n * p.ratio, r0 = row_tile * 8 * NT;
+  if (r0 >= rows) return;
+  const int r1 = min(rows, r0 + 8 * NT);
+  int begin, end;
+  attn_range(p, seq, r0, r1, kTile, &begin, &end);
+  begin += split * p.chunk;
+  if (begin >= end && split) return;  // the join counts the splits that have tokens
+  if (split + 1 < p.splits) end = min(end, begin + p.chunk);  // the last one takes what is left
+  attn_rows<T, D, G, NT>(p, seq, b, head, r0, r1, begin, end, split, p.splits, p.box_rows, smem, full_bar, &abort_flag);
 }
 
 // Joins the splits of a sequence, each read once. kLanes = kJoinLanes: a block a query row, D / 4 threads times kLanes

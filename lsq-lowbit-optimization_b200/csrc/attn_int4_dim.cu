@@ -42,10 +42,26 @@ int run_prefill(const AttnParams& p, unsigned grid, cudaStream_t st) {
              : W4A8_ERR_LAUNCH;
 }
 
+// The rows that the blocks of run_prefill handed over; behind the join.
+template <typename T, int G>
+int run_redo(const AttnParams& p, cudaStream_t st) {
+  constexpr int smem = attn_smem_bytes<D, G, 2>();
+  static PerDevice<int> ready;
+  if (allow_smem(kv_attn_redo_kernel<T, D, G>, smem, ready) != W4A8_OK) return W4A8_ERR_LAUNCH;
+  const unsigned grid = unsigned(p.view.batch) * p.view.heads * p.row_tiles * kRedoParts;
+  return launch_kernel(kv_attn_redo_kernel<T, D, G>, dim3(grid), dim3(kAttnWarps * 32), smem, st, p) == cudaSuccess
+             ? W4A8_OK
+             : W4A8_ERR_LAUNCH;
+}
+
+constexpr int kRedo = -1;  // in place of NT
+
 template <typename T, int G, int NT>
 int run(const AttnParams& p, unsigned grid, cudaStream_t st) {
   if constexpr (NT == 0) {
     return run_prefill<T, G>(p, grid, st);
+  } else if constexpr (NT == kRedo) {
+    return run_redo<T, G>(p, st);
   } else {
     constexpr int smem = attn_smem_bytes<D, G, NT>();
     static PerDevice<int> ready;
@@ -57,7 +73,7 @@ int run(const AttnParams& p, unsigned grid, cudaStream_t st) {
   }
 }
 
-// NT: tiles of eight query rows of a warp, or 0 for the kernel of many rows.
+// NT: tiles of eight query rows of a warp, 0 for the kernel of many rows, or kRedo.
 template <typename T, int NT>
 int by_group(const AttnParams& p, unsigned grid, cudaStream_t st) {
   switch (p.view.group) {
@@ -76,6 +92,7 @@ template <typename T>
 int by_tiles(const AttnParams& p, int n_tiles, unsigned grid, cudaStream_t st) {
   if constexpr (prefill_ok(D, sizeof(T) == 4)) {
     if (n_tiles == 0) return by_group<T, 0>(p, grid, st);
+    if (n_tiles == kRedo) return by_group<T, kRedo>(p, grid, st);
   }
   if constexpr (attn_wide_ok(D, sizeof(T) == 4)) {
     if (n_tiles == 2) return by_group<T, 2>(p, grid, st);
@@ -89,9 +106,12 @@ int by_tiles(const AttnParams& p, int n_tiles, unsigned grid, cudaStream_t st) {
 #define W4A8_CAT(a, b) W4A8_CAT2(a, b)
 int W4A8_CAT(launch_attn_int4_d, W4A8_HEAD_DIM)(const AttnParams& p, int dtype, int n_tiles, unsigned grid,
                                                 cudaStream_t st) {
-  const int rc = dtype == W4A8_F32   ? by_tiles<float>(p, n_tiles, grid, st)
-                 : dtype == W4A8_F16 ? by_tiles<__half>(p, n_tiles, grid, st)
-                                     : by_tiles<__nv_bfloat16>(p, n_tiles, grid, st);
+  auto rows = [&](int tiles) {
+    return dtype == W4A8_F32   ? by_tiles<float>(p, tiles, grid, st)
+           : dtype == W4A8_F16 ? by_tiles<__half>(p, tiles, grid, st)
+                               : by_tiles<__nv_bfloat16>(p, tiles, grid, st);
+  };
+  const int rc = rows(n_tiles);
   if (rc != W4A8_OK) return rc;
   if (p.splits > 1) {
     const int tile_rows = n_tiles ? 8 * n_tiles : kPreRows, tile_tokens = n_tiles ? kTile : kPreTile;
@@ -99,6 +119,10 @@ int W4A8_CAT(launch_attn_int4_d, W4A8_HEAD_DIM)(const AttnParams& p, int dtype, 
                        : dtype == W4A8_F16 ? join<__half>(p, tile_rows, tile_tokens, st)
                                            : join<__nv_bfloat16>(p, tile_rows, tile_tokens, st);
     if (joined != W4A8_OK) return joined;
+  }
+  if (n_tiles == 0) {
+    const int redone = rows(kRedo);
+    if (redone != W4A8_OK) return redone;
   }
   return cudaGetLastError() == cudaSuccess ? W4A8_OK : W4A8_ERR_LAUNCH;
 }

@@ -13,10 +13,11 @@
 // query heads on 8 of 128 channels, bfloat16: 668 us, 823 TFLOP/s (half of the rate of a plain bfloat16 matrix product).
 //
 // All operands are float16. code * scale has at most 11 significant bits, so keys and values are exact
-// there down to scales of 2^-17: for 32 tokens (those of one unpacking warp) whose largest scale is outside
-// [2^-8, 2^12] they are held divided by a power of two, which scores and weights take up again. So all are exact whose
-// scale is 2^-9 of the largest of their 32 or more, and others are off by 2^-17 of that one. A query is
-// brought to a largest magnitude near 2^14 by a power of two. Weights are rounded to 11 bits.
+// there for scales from 2^-17 to 2^12. Where the largest scale of a block's first tile is not within [2^-9, 2^8] they are
+// held divided by a power of two, one for the block's keys and one for its values. A block that meets a scale outside
+// of the range all the same (of a token that its rows see or not) says so, and kv_attn_redo_kernel takes its rows again with
+// the arithmetic of few rows. Otherwise large values, hidden ones even, would set the unit that small ones are lost in. A
+// query is brought to a largest magnitude near 2^14 by a power of two. Weights are rounded to 11 bits.
 //
 // TMEM (512 columns): S of tile 0 and 1 at 0 and 128, their weights over them; O at 256 and 384.
 //
@@ -34,7 +35,6 @@ constexpr int kPreRows = 2 * kPreTile;       // query rows of a block
 constexpr int kPreThreads = 20 * 32;         // 2 x 4 softmax warps, 2 x 4 unpacking warps, 1 issuing warp, 3 idle
 constexpr int kPreIssuer = 16;               // its warp
 constexpr int kPreStages = 2;                // tiles of keys, and of values, in shared memory
-constexpr int kPreUnits = 4;                 // tiles whose units are kept: keys run ahead of the weights by two
 constexpr int kPrePanel = kPreTile * 128;    // 128 rows of 64 channels, swizzled 128-byte rows
 
 template <int D>
@@ -161,12 +161,15 @@ __device__ __forceinline__ uint4 unpack8(uint32_t w, __half2 s) {
                         __hmul2(code_pair_high(y), s)};
   return *reinterpret_cast<const uint4*>(r);
 }
-// 2^e for 32 tokens whose largest scale has the bits `top` (a non-negative float): 1 within [2^-8, 2^12]. Where all
-// are zeros (no tokens there, for one) any unit is right, and the last tile's asks for no rescaling.
-__device__ __forceinline__ float pre_unit(uint32_t top, float last) {
+// The power of two that keys or values are held divided by, from the bits of the largest scale of a block's first tile.
+__device__ __forceinline__ float pre_unit(uint32_t top) {
   const float f = __uint_as_float(top);
-  if (f == 0.0f) return last;
-  return f >= 0x1p-8f && f <= 0x1p12f ? 1.0f : __uint_as_float(max(top & 0x7f800000u, 0x00800000u));
+  return f == 0.0f || (f >= 0x1p-9f && f <= 0x1p8f) ? 1.0f : __uint_as_float(max(top & 0x7f800000u, 0x00800000u));
+}
+
+// All threads of one of the two groups of unpacking warps.
+__device__ __forceinline__ void pre_group_sync(int which) {
+  asm volatile("bar.sync %0, 128;" ::"r"(1 + which) : "memory");
 }
 
 template <typename T>
@@ -215,7 +218,7 @@ __device__ __forceinline__ bool pre_wait_idle(uint64_t* bar, uint32_t parity, vo
 
 struct PreBars {
   uint64_t q_full, k_full[kPreStages], k_empty[kPreStages], v_full[kPreStages], v_empty[kPreStages];
-  uint64_t s_full[2], p_full[2], o_done[2], k_said[kPreUnits];
+  uint64_t s_full[2], p_full[2], o_done[2], said;
 };
 
 template <typename T, int D, int G>
@@ -233,7 +236,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
   // Values that are NaN: the groups that have some, by stage and unpacking warp, and their tokens.
   __shared__ uint32_t nan_any[kPreStages][4], nan_tokens[kPreStages][kGroups][4];
   __shared__ float row_mul[kPreRows];
-  __shared__ __align__(16) float k_unit[kPreUnits][4], v_unit[kPreUnits][4];
+  __shared__ uint32_t first_top[2][4];  // largest scale of the first tile, of each unpacking warp
+  __shared__ float units[2];            // of keys and values
+  __shared__ int handover;
   pdl_trigger();
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   const uint32_t sbase = smem_u32(smem);
@@ -244,6 +249,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
   if (warp == kPreIssuer) {
     if (lane == 0) {
       abort_flag = 0;
+      handover = 0;
       mbar_init(&bars.q_full, 8);
       for (int i = 0; i < kPreStages; ++i) {
         mbar_init(&bars.k_full[i], 4);
@@ -256,7 +262,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
         mbar_init(&bars.p_full[i], 4);
         mbar_init(&bars.o_done[i], 1);
       }
-      for (int i = 0; i < kPreUnits; ++i) mbar_init(&bars.k_said[i], 4);
+      mbar_init(&bars.said, 2);
       fence_mbarrier_init();
     }
   }
@@ -318,9 +324,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
     uint64_t *full = which ? bars.v_full : bars.k_full, *empty = which ? bars.v_empty : bars.k_empty;
     uint8_t* buffers = smem + (which ? Smem::kV : Smem::kK);
     const uint32_t my_codes = sbase + Smem::kCodes + which * Smem::kCodeBytes;
-    float(*units)[4] = which ? v_unit : k_unit;
     __nv_bfloat16 cur_s[kGroups], nxt_s[kGroups];
-    float unit = 0x1p-126f;  // of this warp's 32 tokens
     auto page_of = [&](int j) {
       const int t = begin + j * kPreTile + r;
       return j < all_tiles && t < end ? kv_page_id(v, b, kv_page_of(v, t)) : -1;
@@ -338,28 +342,43 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
     };
     fetch(0, page_of(0));
     int id = page_of(1);
+    float inv;  // of the unit
+    {
+      uint32_t top = 0;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const float f = fabsf(__bfloat162float(nxt_s[g]));
+        if (f <= 3.4e38f) top = max(top, __float_as_uint(f));
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) first_top[which][slice] = top;
+      pre_group_sync(which);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = max(top, first_top[which][i]);
+      const float unit = pre_unit(top);
+      inv = __frcp_rn(unit);
+      if (r == 0) {
+        units[which] = unit;
+        mbar_arrive(&bars.said);
+      }
+    }
     for (int j = 0; j < all_tiles; ++j) {
 #pragma unroll
       for (int k = 0; k < kGroups; ++k) cur_s[k] = nxt_s[k];
       fetch(j + 1, id);  // a tile ahead, and its page two
       id = page_of(j + 2);
       const int st = j % kPreStages;
-      uint32_t top = 0, any = 0;
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        const float f = __bfloat162float(cur_s[g]);
-        if (fabsf(f) <= 3.4e38f) top = max(top, __float_as_uint(f) & 0x7fffffffu);
-      }
-      unit = pre_unit(__reduce_max_sync(0xffffffffu, top), unit);
-      const float inv = __frcp_rn(unit);
+      uint32_t any = 0;
+      bool unfit = false;
       cp_async_wait<1>();
       if (!__all_sync(0xffffffffu, pre_wait_idle(&empty[st], ((j / kPreStages) & 1) ^ 1, &abort_flag))) break;
-      if (lane == 0) units[j % kPreUnits][slice] = unit;
       uint8_t* dst = buffers + st * Smem::kTileBytes;
       const uint32_t src = my_codes + st * 2 * Smem::kCodeBytes;
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
-        float f = __bfloat162float(cur_s[g]) * inv;
+        const float scale = __bfloat162float(cur_s[g]);
+        float f = scale * inv;
+        unfit |= scale != 0.0f && fabsf(scale) <= 3.4e38f && !(fabsf(f) >= 0x1p-17f && fabsf(f) <= 0x1p12f);
         if (which) {
           // NaN values (and infinite ones) become zeros here; the rows that see them get NaN at the end.
           const bool bad = !(fabsf(f) <= 3.4e38f);
@@ -378,12 +397,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
         }
       }
       if (which && lane == 0) nan_any[st][slice] = any;
+      if (unfit) handover = 1;
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&full[st]);
-        if (!which) mbar_arrive(&bars.k_said[j % kPreUnits]);
-      }
+      if (lane == 0) mbar_arrive(&full[st]);
     }
     cp_async_wait<0>();
   } else if (warp >= kPreIssuer) {
@@ -530,15 +547,16 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
     const int lo = p.window > 0 ? max(0, max(0, pos) - p.window + 1) : 0;
     const int hi = pos < 0 || !mine ? 0 : p.causal ? min(end, pos + 1) : end;
     const uint32_t quad = uint32_t(warp & 3) << 21, s_addr = tmem + s * 128 + quad, o_addr = tmem + 256 + s * 128 + quad;
-    float m = kNegInf, l = 0.0f, v_ref = 0x1p-126f;
+    float m = kNegInf, l = 0.0f;
     uint32_t nan_groups = 0;
-    bool ok = true;
-    for (int j = 0; j < tiles[s]; ++j) {
-      // What the unpacking warps say about the tile (units and NaN values) is read before the weights are
+    bool ok = __all_sync(0xffffffffu, pre_wait(&bars.said, 0, &abort_flag));
+    const float m32 = fmaxf(mul * units[0], 1.2e-38f);  // a score's factor; positive, for the hidden scores' -inf
+    const uint64_t mul2 = pair2(m32, m32);
+    for (int j = 0; ok && j < tiles[s]; ++j) {
+      // What the unpacking warps say about the tile (NaN values) is read before the weights are
       // handed over: until the products with them are done it is not written over.
       const int st = j % kPreStages;
       if (!__all_sync(0xffffffffu, pre_wait(&bars.s_full[s], j & 1, &abort_flag) &&
-                                       pre_wait(&bars.k_said[j % kPreUnits], (j / kPreUnits) & 1, &abort_flag) &&
                                        pre_wait(&bars.v_full[st], (j / kPreStages) & 1, &abort_flag))) {
         ok = false;
         break;
@@ -547,10 +565,6 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
       const int t0 = begin + j * kPreTile;
       const int from = max(lo - t0, 0), to = min(hi - t0, kPreTile);  // columns that this row sees
       const bool partial = __any_sync(0xffffffffu, from > 0 || to < kPreTile);
-      const float* ku = k_unit[j % kPreUnits];
-      const float* vu = v_unit[j % kPreUnits];
-      const float v_next = fmaxf(v_ref, fmaxf(fmaxf(vu[0], vu[1]), fmaxf(vu[2], vu[3])));
-      const bool plain = fminf(fminf(vu[0], vu[1]), fminf(vu[2], vu[3])) == v_next;
       if (nan_any[st][0] | nan_any[st][1] | nan_any[st][2] | nan_any[st][3]) {
         for (int g = 0; g < kGroups; ++g)
           for (int k = from; k < to; ++k)
@@ -568,8 +582,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
         const uint32_t seen = bits_between(from - c * 32, to - c * 32);
 #pragma unroll
         for (int k = 0; k < 32; ++k) m = fmaxf(m, seen >> k & 1 ? y[k] : kNegInf);
-        m *= fmaxf(mul * ku[c], 1.2e-38f);
-        v_ref = v_next;
+        m *= m32;
       }
       uint32_t w[kPreTile / 2];
       float sum;
@@ -596,8 +609,6 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
                 if (c * 32 + k < from || c * 32 + k >= to) y[k] = kNegInf;
             }
           }
-          const float m32 = fmaxf(mul * ku[c], 1.2e-38f);  // positive, for the hidden scores' -inf
-          const uint64_t mul2 = pair2(m32, m32);
           float t[2] = {kNegInf, kNegInf};
 #pragma unroll
           for (int k = 0; k < 32; k += 2) t[k / 2 & 1] = fmaxf(t[k / 2 & 1], fmaxf(y[k], y[k + 1]));
@@ -615,7 +626,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
         float a, d;
         unpair2(add2(acc0, acc1), a, d);
         sum = a + d;
-        again = !again && __any_sync(0xffffffffu, top > m + 8.0f || v_next != v_ref);
+        again = !again && __any_sync(0xffffffffu, top > m + 8.0f);
         if (again) {
           const float next = fmaxf(m, top);
           const float c = next == kNegInf ? 1.0f : exp2_approx(m - next);
@@ -624,33 +635,23 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
           if (j) {
             ok = __all_sync(0xffffffffu, pre_wait(&bars.o_done[s], (j - 1) & 1, &abort_flag));
             tc_fence_after();
-            const float cv = c * __fdiv_rn(v_ref, v_next);
 #pragma unroll 1
             for (int k = 0; ok && k < D / 16; ++k) {
               float y[16];
               tmem_ld16f(o_addr + k * 16, y);
               tmem_ld_wait16(y);
 #pragma unroll
-              for (int e = 0; e < 16; ++e) y[e] *= cv;
+              for (int e = 0; e < 16; ++e) y[e] *= c;
               tmem_st16(o_addr + k * 16, reinterpret_cast<const uint32_t(&)[16]>(y));
             }
           }
         }
       } while (again);
       if (!ok) break;
-      if (!plain) {  // weights take up their values' units
-#pragma unroll
-        for (int k = 0; k < kPreTile / 2; ++k) {
-          const __half2 f = __float2half2_rn(__fdiv_rn(vu[k / 16], v_next));
-          const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&w[k]), f);
-          w[k] = *reinterpret_cast<const uint32_t*>(&y);
-        }
-      }
 #pragma unroll
       for (int k = 0; k < kPreTile / 2; k += 16)
         tmem_st16(s_addr + k, *reinterpret_cast<const uint32_t(*)[16]>(w + k));
       l += sum;
-      v_ref = v_next;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -661,7 +662,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
     if (!ok && lane == 0) atomicOr(v.err, kErrTimeoutEpilogue);
     tc_fence_after();
     const long long at = (long long)(seq.row0 + token) * p.q_heads + qh;
-    const float inv = p.splits > 1 ? v_ref : l == 0.0f ? 0.0f : __frcp_rn(l) * v_ref;
+    const float inv = p.splits > 1 ? units[1] : l == 0.0f ? 0.0f : __frcp_rn(l) * units[1];
 #pragma unroll
     for (int k = 0; k < D / 32; ++k) {
       float x[32];
@@ -702,10 +703,39 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
     tc_fence_before();
   }
   __syncthreads();
+  if (threadIdx.x == 0) p.handover[blockIdx.x] = handover;
   if (warp == kPreIssuer) {
     tc_fence_after();
     __syncwarp();
     tmem_dealloc(tmem, 512);
+  }
+}
+
+// The rows of blocks whose scales are too far apart for float16, by the arithmetic of few rows: kRedoParts blocks for each of the
+// prompt kernel's tiles of rows, which all leave at once where no piece of the tile was handed over.
+constexpr int kRedoParts = 4;
+
+template <typename T, int D, int G>
+__global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_sm(D, 2, false))
+    kv_attn_redo_kernel(const __grid_constant__ AttnParams p) {
+  constexpr int kRows = 16;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  pdl_trigger();
+  const unsigned tile = blockIdx.x / kRedoParts, part = blockIdx.x % kRedoParts;
+  pdl_wait();
+  int redo = 0;
+  for (int s = 0; s < p.splits; ++s) redo |= p.handover[(long long)tile * p.splits + s];
+  if (!redo) return;
+  const BlockWork work = block_work(p, tile * unsigned(p.splits));
+  const int row_tile = p.row_tiles - 1 - work.row_tile;  // as the prompt kernel counts them
+  const KvSeq seq = kv_seq(p.view, work.b);
+  const int rows = min(seq.n * p.ratio, (row_tile + 1) * kPreRows);
+  for (int r0 = row_tile * kPreRows + int(part) * kRows; r0 < rows; r0 += kRedoParts * kRows) {
+    const int r1 = min(rows, r0 + kRows);
+    int begin, end;
+    attn_range(p, seq, r0, r1, kTile, &begin, &end);
+    attn_rows<T, D, G, kRows / 8>(p, seq, work.b, work.head, r0, r1, begin, end, 0, 1, 0, smem, nullptr, nullptr);
+    __syncthreads();  // the results have left the shared memory that the next rows' stages take
   }
 }
 

@@ -15,11 +15,14 @@ def attention_and_bound(q, setup, dtype, scale, causal=True, window=0, many=Fals
 
     To first order an output is off by sum_t p_t (|v_t| + |o|) e_t, where e_t is what the weight of token t is off by:
     * its score. For two-byte queries sums of products with codes of up to 15 are rounded d / 16 + 5 times to no less than 22
-      bits of the largest, 16 scale sum |q| s. A float32 query is held in 23 bits of its largest magnitude, met by codes of up
+      bits of the largest, 16 scale sum |q| s. Each product is cut off at 2^-25 of the largest of its step, for which the tensor cores
+      take a subnormal code n 2^-24 as 2^-14 (measured: beside n 2^-24 times 2^13, products of 2^-26 are kept, of 2^-27 not). The
+      query is scaled to [2^13, 2^14), so that is 2^-26 of 2^-1 2^24 = 1/4 where the largest |q| stands as 2^13 or more: off by
+      2^-15 scale max |q| s for each channel. A float32 query is held in 23 bits of its largest magnitude, met by codes of up
       to 8, and three sums are rounded to 24 bits;
     * the exponential and its argument, 2^-21 (1 + |score|);
     * its own rounding: WEIGHT, or with many rows 2^-11 and, relative to the row's largest weight, 2^-32 (the smallest float16 is
-      2^-24, and the reference weight 2^7).
+      2^-24, and the reference weight 2^7). Weights below 2^-126 of the largest are zeros.
     Sums over the tokens take a step for 16 of them and each term, each off by 2^-22 of what was added up."""
     want, lse = kvo.attention(q, setup.cache, setup.table, setup.lens, setup.cu, scale, causal, window)
     off, lse_off = np.zeros(want.shape), np.zeros(lse.shape)
@@ -50,10 +53,11 @@ def attention_and_bound(q, setup, dtype, scale, causal=True, window=0, many=Fals
                     e = 8 * abs(scale) * (s @ (np.abs(x).max() * 2.0 ** -23 + np.abs(x) * 3 * 2.0 ** -24))
                 else:
                     e = 16 * abs(scale) * (s @ np.abs(x)) * (d / 16 + 5) * 2.0 ** -22
+                    e = e + 2.0 ** -15 * abs(scale) * np.abs(x).max() * s.sum(-1)
                 e = e + 2.0 ** -21 * (1 + np.abs(score))
                 lse_off[row, h] = (p * e).sum() + 2.0 ** -21 * (1 + abs(lse[row, h]))
                 e = e + (2.0 ** -11 if many else WEIGHT[dtype]) + (seen.sum() / 16 + 4) * terms * 2.0 ** -22
-                least = 2.0 ** -32 * p.max() if many else 0.0
+                least = (2.0 ** -32 if many else 2.0 ** -126) * p.max()
                 off[row, h] = (p * e + least) @ np.abs(vs) + (p * e).sum() * np.abs(want[row, h])
     return want, lse, off, lse_off
 

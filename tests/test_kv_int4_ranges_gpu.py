@@ -1,0 +1,117 @@
+"""Attention over a 4-bit cache whose scales are far apart: what a row does not see, or gives no weight, takes nothing from
+what it does see."""
+import numpy as np
+import pytest
+import torch
+
+import int4_int8_ext as ext
+from tests import kv_bounds
+from tests.kv_helpers import Setup, offsets, typed
+
+pytestmark = pytest.mark.gpu
+
+
+def _filled(s, k, v):
+    s.cache.write(k, v, s.table, s.lens, offsets(s.lens))
+    s.tensors = s.upload()
+
+
+def _run(cuda, s, dtype, scale, q_heads=2, **options):
+    idx, cu = s.index()
+    q, qt = typed(s.g.standard_normal((s.cu[-1], q_heads, s.tensors[0].shape[3] * 2)), dtype)
+    return q, ext.attention_int4_kv(qt.to(cuda), *s.tensors, *idx, cu_q=cu, max_q=max(s.news), scale=scale, return_lse=True,
+                                    **options)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("n", [12, 150])  # few rows, and many
+@pytest.mark.parametrize("exp", [14, 20, 30, 60])
+@pytest.mark.parametrize("which", ["keys", "values"])
+@pytest.mark.parametrize("d,group", [(64, 32), (128, 64), (96, 32)])
+def test_hidden_tokens_of_any_size_take_nothing(cuda, dtype, n, exp, which, d, group):
+    """Tokens 2^exp times as large as the others, hidden from rows before them (causality) and behind them (the window)."""
+    length, bad, window = 300, 200, 40
+    s = Setup(exp + n, [length], [n], 1, d, group, 16, cuda)
+    k, v = (typed(s.g.standard_normal((length, 1, d)), "bf16")[0] for _ in range(2))
+    (k if which == "keys" else v)[bad - 3:bad] *= 2.0 ** exp
+    _filled(s, k, v)
+    pos = np.arange(length - n, length)
+    hidden = (pos < bad - 3) | (pos >= bad - 1 + window)
+    assert hidden.any()
+    q, (out, lse) = _run(cuda, s, dtype, 0.05, window=window)
+    want, want_lse, off, lse_off = kv_bounds.attention_and_bound(q, s, dtype, 0.05, True, window, many=n > 32)
+    got = out.double().cpu().numpy()
+    half = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11}[dtype]
+    err, tol = np.abs(got - want)[hidden], (off + half * (np.abs(want) + off) + 2.0 ** -25)[hidden]
+    assert np.all(err <= tol), (err / tol).max()
+    assert np.all(np.abs(lse.double().cpu().numpy() - want_lse)[hidden] <= lse_off[hidden])
+
+
+@pytest.mark.parametrize("n", [12, 150])
+@pytest.mark.parametrize("exp", [13, 24, 50])
+def test_seen_tokens_without_weight_take_nothing(cuda, n, exp):
+    """Large values whose tokens' scores are far below the others'."""
+    s = Setup(exp, [300], [n], 1, 64, 32, 16, cuda)
+    k, v = (s.g.standard_normal((300, 1, 64)) for _ in range(2))
+    large = np.arange(300) % 50 == 7
+    k[:, 0, 0] = np.where(large, -7.0, 0.5)
+    v = v * np.where(large, 2.0 ** exp, 1)[:, None, None]
+    k, v = (typed(x, "bf16")[0] for x in (k, v))
+    _filled(s, k, v)
+    idx, cu = s.index()
+    q, qt = s.g.standard_normal((n, 2, 64)) * 0.1, None
+    q[..., 0] = 30.0  # a large token's score is 225 below the others'
+    q, qt = typed(q, "bf16")
+    out, lse = ext.attention_int4_kv(qt.to(cuda), *s.tensors, *idx, scale=1.0, return_lse=True)
+    kv_bounds.check(q, out, lse, s, "bf16", 1.0, many=n > 32)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("n", [12, 150])
+@pytest.mark.parametrize("window", [0, 64])
+@pytest.mark.parametrize("ratio", [0.1, 10.0])
+def test_values_that_shrink_or_grow(cuda, dtype, n, window, ratio):
+    """Values ten times smaller, or larger, every 60 tokens; with a window only the last ones are seen."""
+    s = Setup(41, [600], [n], 2, 64, 32, 16, cuda)
+    size = ratio ** (np.arange(600) // 60 - (9 if ratio > 1 else 0))
+    k, v = (s.g.standard_normal((600, 2, 64)) for _ in range(2))
+    k, v = typed(k, "bf16")[0], typed(v * 1e4 * size[:, None, None], "bf16")[0]
+    _filled(s, k, v)
+    q, (out, lse) = _run(cuda, s, dtype, 0.05, q_heads=4, window=window)
+    kv_bounds.check(q, out, lse, s, dtype, 0.05, True, window, many=n > 32)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("exp", [-40, -22, -14, -9, 8, 14])
+def test_caches_of_any_size_that_is_even(cuda, dtype, exp):
+    """All scales near 2^exp, some of them on either side of a power of two."""
+    s = Setup(43, [300], [150], 1, 128, 64, 16, cuda)
+    k, v = (typed(s.g.standard_normal((300, 1, 128)) * np.exp2(s.g.integers(-1, 2, (300, 1, 1)) + float(exp)), "bf16")[0]
+            for _ in range(2))
+    if dtype == "f16":
+        v = typed(v * 2.0 ** (-exp), "bf16")[0]  # outputs that the type can hold
+    _filled(s, k, v)
+    scale = 0.05 * 2.0 ** -exp
+    q, (out, lse) = _run(cuda, s, dtype, scale)
+    kv_bounds.check(q, out, lse, s, dtype, scale, many=True)
+
+
+@pytest.mark.parametrize("batch,lens", [(1, [5000]), (3, [3000, 100, 1500])])
+def test_large_hidden_values_in_calls_that_are_split(cuda, batch, lens):
+    """A long cache, few row tiles: the pieces of a sequence meet large values in some places only."""
+    news = [min(n, 70) for n in lens]
+    s = Setup(47, lens, news, 1, 64, 32, 16, cuda)
+    total = sum(lens)
+    k, v = (typed(s.g.standard_normal((total, 1, 64)), "bf16")[0] for _ in range(2))
+    for b, at in enumerate(offsets(lens)[1:]):
+        v[at - 3] *= 2.0 ** 40  # hidden from all rows but the last three
+    _filled(s, k, v)
+    q, (out, lse) = _run(cuda, s, "f16", 0.05, max_len=max(lens))
+    want, want_lse, off, lse_off = kv_bounds.attention_and_bound(q, s, "f16", 0.05, many=True)
+    ok = np.ones(len(q), bool)
+    for at in s.cu[1:]:
+        ok[at - 3:at] = False
+    got = out.double().cpu().numpy()
+    err, tol = np.abs(got - want)[ok], (off + 2.0 ** -11 * (np.abs(want) + off) + 2.0 ** -25)[ok]
+    assert np.all(err <= tol), (err / tol).max()
+    assert np.all(np.abs(lse.double().cpu().numpy() - want_lse)[ok] <= lse_off[ok])
