@@ -17,7 +17,9 @@
 // held divided by a power of two, one for the block's keys and one for its values. A block that meets a scale outside
 // of the range all the same (of a token that its rows see or not) says so, and kv_attn_redo_kernel takes its rows again with
 // the arithmetic of few rows. Otherwise large values, hidden ones even, would set the unit that small ones are lost in. A
-// query is brought to a largest magnitude near 2^14 by a power of two. Weights are rounded to 11 bits.
+// query is brought to a largest magnitude near 2^14 by a power of two. Weights are rounded to 11 bits, and to multiples of
+// 2^-31 of the row's largest: that is what a long tail of small weights beside one large is off by. Two float16 terms would need
+// twice the products and registers that a row does not have; error of float16 outputs 2.7e-4, of their own rounding 2.0e-4.
 //
 // TMEM (512 columns): S of tile 0 and 1 at 0 and 128, their weights over them; O at 256 and 384.
 //
@@ -53,6 +55,10 @@ constexpr int prefill_smem_bytes() {
   // The base is rounded up to 1024; more than half of an SM's, since a block takes all of its TMEM.
   return (PreSmem<D>::kBytes > 118 * 1024 ? PreSmem<D>::kBytes : 118 * 1024) + 1024;
 }
+
+// Weights are 2^(score - m). m is set so that the largest is 2^kPreHigh, and raised when one would pass 2^kPreRaise: float16
+// goes up to 2^16, and what is small keeps bits down to 2^-24, which is 2^-31 of the largest or less.
+constexpr float kPreHigh = 7.0f, kPreRaise = 15.0f;
 
 // Bits [from, to) of 32, either of them anywhere.
 __device__ __forceinline__ uint32_t bits_between(int from, int to) {
@@ -571,8 +577,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
             if (nan_tokens[st][g][k >> 5] >> (k & 31) & 1) nan_groups |= 1u << g;
       }
       // Weights for the reference m of the tiles before, and the largest score on the way. Only when that
-      // passes m by more than 8 (or at the first tile) m is raised, the output rescaled and the row done again, so
-      // most tiles take one pass, and weights stay below 2^8. They are held in registers until then, since
+      // passes m by more than kPreRaise (or at the first tile) m is raised, the output rescaled and the row done again, so
+      // most tiles take one pass. They are held in registers until then, since
       // they go where the scores are. The next 32 columns are loaded while these are worked on.
       if (kQuickEdges && j == 0) {  // nothing to go by yet: the largest of 32 columns that the rows of the warp see
         const int c = min(max(__shfl_sync(0xffffffffu, from, 31), 0), kPreTile - 1) / 32;
@@ -582,7 +588,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
         const uint32_t seen = bits_between(from - c * 32, to - c * 32);
 #pragma unroll
         for (int k = 0; k < 32; ++k) m = fmaxf(m, seen >> k & 1 ? y[k] : kNegInf);
-        m *= m32;
+        m = m * m32 - kPreHigh;
       }
       uint32_t w[kPreTile / 2];
       float sum;
@@ -626,9 +632,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
         float a, d;
         unpair2(add2(acc0, acc1), a, d);
         sum = a + d;
-        again = !again && __any_sync(0xffffffffu, top > m + 8.0f);
+        again = !again && __any_sync(0xffffffffu, top > m + kPreRaise);
         if (again) {
-          const float next = fmaxf(m, top);
+          const float next = fmaxf(m, top - kPreHigh);
           const float c = next == kNegInf ? 1.0f : exp2_approx(m - next);
           m = next;
           l *= c;

@@ -115,3 +115,22 @@ def test_large_hidden_values_in_calls_that_are_split(cuda, batch, lens):
     err, tol = np.abs(got - want)[ok], (off + 2.0 ** -11 * (np.abs(want) + off) + 2.0 ** -25)[ok]
     assert np.all(err <= tol), (err / tol).max()
     assert np.all(np.abs(lse.double().cpu().numpy() - want_lse)[ok] <= lse_off[ok])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("n", [12, 150])
+def test_a_sink_with_small_values_and_a_long_tail(cuda, dtype, n):
+    """One token takes nearly all of the weight and has zeros for values: what is left comes from equal small weights, of
+    2^-20 to 2^-24 of the largest."""
+    s = Setup(53, [2000], [n], 1, 64, 32, 16, cuda)
+    k, v = np.zeros((2000, 1, 64)), 1 + 0.1 * s.g.standard_normal((2000, 1, 64))
+    k[0, 0, 0] = 7.0
+    v[0] = 0
+    k, v = (typed(x, "bf16")[0] for x in (k, v))
+    _filled(s, k, v)
+    idx, cu = s.index()
+    q = np.zeros((n, 2, 64))
+    q[:, 0, 0], q[:, 1, 0] = np.linspace(13.9, 16.6, n), np.linspace(14.3, 16.1, n)  # scores of the sink, in nats
+    q, qt = typed(q, dtype)
+    out, lse = ext.attention_int4_kv(qt.to(cuda), *s.tensors, *idx, scale=1.0 / 7, return_lse=True)
+    kv_bounds.check(q, out, lse, s, dtype, 1.0 / 7, many=n > 32)
