@@ -272,7 +272,7 @@ constexpr int kClearBlocks = 8;
 template <typename T>
 __device__ void attn_clear_outside(const AttnParams& p, int slice, int slices) {
   const KvView& v = p.view;
-  const int first = min(max(__ldg(v.cu_q), 0), v.rows), last = min(max(__ldg(v.cu_q + v.batch), first), v.rows);
+  const int first = min(max(v.cu_q[0], 0), v.rows), last = min(max(v.cu_q[v.batch], first), v.rows);
   const int n = first + v.rows - last, from = int((long long)n * slice / slices),
             to = int((long long)n * (slice + 1) / slices);
   attn_clear_rows<T>(p, from, min(to, first), 0, p.q_heads);
@@ -369,7 +369,7 @@ __device__ __forceinline__ void attn_rows(const AttnParams& p, const KvSeq& seq,
   int ahead = 0;  // page of token l of the tile that load_tile copies next
   auto ask_page = [&](int j) {
     const int t = begin + (warp + j * kAttnWarps) * kTile + lane;
-    ahead = t < end ? __ldg(table + kv_page_of(v, t)) : 0;
+    ahead = t < end ? table[kv_page_of(v, t)] : 0;
   };
   auto load_tile = [&](int j) {
     if (j < my_tiles) {
@@ -436,7 +436,7 @@ __device__ __forceinline__ void attn_rows(const AttnParams& p, const KvSeq& seq,
 #pragma unroll
       for (int s = 0; s < kSegs; ++s) {
         if (sizeof(T) == 2 && p.q_vec) {
-          const uint4 w = __ldg(reinterpret_cast<const uint4*>(src + s * 32));
+          const uint4 w = *reinterpret_cast<const uint4*>(src + s * 32);
           const T* e = reinterpret_cast<const T*>(&w);
 #pragma unroll
           for (int k = 0; k < 8; ++k) x[s][k] = to_f32<T>(e[k]);

@@ -8,6 +8,9 @@
 // Every index that comes from device memory (block table, lengths, row offsets) is checked
 // here before it is used: a bad one reads as zeros, is not written to, and sets
 // kErrCacheIndex in the device error word.
+//
+// All of it is read by ordinary loads: a block may be resident while the kernel ahead, which writes the cache, the rows or
+// the tables, still runs (launch.cuh), and the read-only path promises data that nobody writes in a kernel's life.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -68,8 +71,8 @@ __device__ __forceinline__ KvSeq kv_seq(const KvView& v, int b) {
   KvSeq s;
   bool bad = false;
   if (v.cu_q) {
-    s.row0 = __ldg(v.cu_q + b);
-    const int end = __ldg(v.cu_q + b + 1);
+    s.row0 = v.cu_q[b];
+    const int end = v.cu_q[b + 1];
     if (s.row0 < 0 || end < s.row0 || end > v.rows) {
       bad = true;
       s.row0 = 0;
@@ -81,7 +84,7 @@ __device__ __forceinline__ KvSeq kv_seq(const KvView& v, int b) {
     s.n = v.rows / v.batch;
     s.row0 = b * s.n;
   }
-  s.len = __ldg(v.seq_lens + b);
+  s.len = v.seq_lens[b];
   const int cap = kv_capacity(v);
   if (s.len < 0 || s.len > cap) {
     bad = true;
@@ -93,7 +96,7 @@ __device__ __forceinline__ KvSeq kv_seq(const KvView& v, int b) {
 
 // Page of token t (0 <= t < capacity) of sequence b, or -1 where the table names none.
 __device__ __forceinline__ int kv_page_id(const KvView& v, int b, int p) {
-  const int id = __ldg(v.table + (long long)b * v.table_ld + p);
+  const int id = v.table[(long long)b * v.table_ld + p];
   if (unsigned(id) >= unsigned(v.pages)) {
     kv_error(v);
     return -1;

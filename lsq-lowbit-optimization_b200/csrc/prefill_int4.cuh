@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
       cp_async_commit();
       const __nv_bfloat16* s_from = scales + (id < 0 ? 0 : id * v.s_page + at * v.s_tok);
 #pragma unroll
-      for (int k = 0; k < kGroups; ++k) nxt_s[k] = id < 0 ? __ushort_as_bfloat16(0) : __ldg(s_from + k);
+      for (int k = 0; k < kGroups; ++k) nxt_s[k] = id < 0 ? __ushort_as_bfloat16(0) : s_from[k];
     };
     fetch(0, page_of(0));
     int id = page_of(1);
@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
           const T* src = static_cast<const T*>(p.q) + (seq.row0 + at.token) * p.q_row +
                          (head * p.ratio + at.head) * p.q_head + c * 8;
           if (p.q_vec) {
-            to[k] = __ldg(reinterpret_cast<const uint4*>(src));
+            to[k] = *reinterpret_cast<const uint4*>(src);
           } else {
             T* e = reinterpret_cast<T*>(&to[k]);
 #pragma unroll
