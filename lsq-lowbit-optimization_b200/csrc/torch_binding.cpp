@@ -67,6 +67,11 @@ void check_index(const Tensor& t, const char* name, int dim, const Tensor& like)
   require(t.size(-1) <= 1 || t.stride(-1) == 1, name, " must have a contiguous last dimension");
 }
 
+void check_constant(const Tensor& t, const char* name) {
+  require(!(t.requires_grad() && c10::GradMode::is_enabled()), name,
+          " requires a gradient, which the 4-bit cache does not have: use torch.no_grad()");
+}
+
 void check_rows(const Tensor& t, const char* name, int64_t heads, const Tensor& k_codes) {
   require(t.device() == k_codes.device(), name, " must be on the cache's device");
   require(t.dim() == 3, name, " must be rank-3 [rows, heads, head_dim]");
@@ -74,8 +79,7 @@ void check_rows(const Tensor& t, const char* name, int64_t heads, const Tensor& 
   require(t.size(2) == 2 * k_codes.size(3), name, " must have the cache's head_dim");
   require(heads < 0 || t.size(1) == heads, name, " must have the cache's heads");
   require(t.numel() == 0 || t.stride(2) == 1, name, " must have a contiguous last dimension");
-  require(!(t.requires_grad() && c10::GradMode::is_enabled()), name,
-          " requires a gradient, which the 4-bit cache does not have: use torch.no_grad()");
+  check_constant(t, name);
 }
 
 void check_codes(const Tensor& k_codes) {
@@ -99,6 +103,7 @@ w4a8_kv_cache make_cache(const Tensor& k_codes, const Tensor& v_codes, const Ten
               scales.size(3) == 2,
           "scales must be rank-5 [pages, kv_heads, page_size, 2, head_dim / group]");
   require(scales.scalar_type() == at::kBFloat16, "scales must be bfloat16");
+  check_constant(scales, "scales");
   const int64_t groups = scales.size(4);
   require(groups > 0 && (32 * groups == d || 64 * groups == d || 128 * groups == d),
           "scales must hold one value for 32, 64 or 128 channels");
@@ -156,6 +161,8 @@ void kv_write(const Tensor& k, const Tensor& v, const Tensor& k_codes, const Ten
   check_codes(k_codes);
   check_rows(k, "k", k_codes.size(1), k_codes);
   check_rows(v, "v", k_codes.size(1), k_codes);
+  if (k_step) check_constant(*k_step, "k_step");
+  if (v_step) check_constant(*v_step, "v_step");
   require(v.size(0) == k.size(0) && v.scalar_type() == k.scalar_type(), "k and v must have the same shape and type");
   const int64_t rows = k.size(0);
   const w4a8_kv_cache c = make_cache(k_codes, v_codes, scales, block_table, seq_lens, cu_q, rows);
