@@ -70,6 +70,7 @@ void check_index(const Tensor& t, const char* name, int dim, const Tensor& like)
 void check_constant(const Tensor& t, const char* name) {
   require(!(t.requires_grad() && c10::GradMode::is_enabled()), name,
           " requires a gradient, which the 4-bit cache does not have: use torch.no_grad()");
+  require(!t._fw_grad(0).defined(), name, " has a forward-mode tangent, which the 4-bit cache does not carry");
 }
 
 void check_rows(const Tensor& t, const char* name, int64_t heads, const Tensor& k_codes) {

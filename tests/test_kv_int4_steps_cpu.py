@@ -27,3 +27,19 @@ def test_refuses_scales_that_require_a_gradient():
                  lambda: ext.attention_int4_kv(x, **c)):
         with pytest.raises(RuntimeError, match="scales requires a gradient"):
             call()
+
+
+def test_refuses_forward_mode_tangents():
+    """They would be dropped, also under no_grad."""
+    import torch.autograd.forward_ad as fwd
+
+    x, c = torch.zeros(4, 2, 64), _cache()
+    with fwd.dual_level(), torch.no_grad():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        step = fwd.make_dual(torch.ones(2, 2), torch.ones(2, 2))
+        for call, name in ((lambda: ext.kv_cache_write_int4(dual, x, **c), "k"),
+                           (lambda: ext.kv_cache_write_int4(x, dual, **c), "v"),
+                           (lambda: ext.kv_cache_write_int4(x, x, **c, k_step=step), "k_step"),
+                           (lambda: ext.attention_int4_kv(dual, **c), "q")):
+            with pytest.raises(RuntimeError, match=name + " has a forward-mode tangent"):
+                call()
