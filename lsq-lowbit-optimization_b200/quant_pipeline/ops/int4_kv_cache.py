@@ -20,7 +20,7 @@ class Int4KVCache(nn.Module):
     ``cu_q`` int32 [batch + 1]; the rows given are the last tokens of their sequences
     (``int4_int8_ext.kv_cache_write_int4``). Buffers move and are saved with the module. ``k_step`` and
     ``v_step`` (float32 [kv_heads, head_dim / group_size]), if given, are learned LSQ steps that take
-    the place of each row's own scales. ``half()``, ``to(dtype)`` and the like on a model that holds the cache
+    the place of each row's own scales; the cache keeps a copy of them on its device, without gradients. ``half()``, ``to(dtype)`` and the like on a model that holds the cache
     leave its types as they are. Inference only."""
 
     def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, group_size: int = 64,
@@ -39,8 +39,13 @@ class Int4KVCache(nn.Module):
         self.register_buffer("v_codes", torch.zeros(codes, dtype=torch.uint8, device=device))
         self.register_buffer("scales", torch.zeros((num_pages, kv_heads, page_size, 2, head_dim // group_size),
                                                    dtype=torch.bfloat16, device=device))
-        self.register_buffer("k_step", k_step)
-        self.register_buffer("v_step", v_step)
+        shape = (kv_heads, head_dim // group_size)
+        for name, step in (("k_step", k_step), ("v_step", v_step)):
+            if step is not None:
+                if not isinstance(step, torch.Tensor) or step.dtype != torch.float32 or tuple(step.shape) != shape:
+                    raise ValueError(f"{name} must be float32 [kv_heads, head_dim / group_size]")
+                step = step.detach().to(self.scales.device, copy=True).contiguous()
+            self.register_buffer(name, step)
 
     def _apply(self, fn, *args, **kwargs):
         def moved(t: torch.Tensor) -> torch.Tensor:

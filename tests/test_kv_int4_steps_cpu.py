@@ -43,3 +43,29 @@ def test_refuses_forward_mode_tangents():
                            (lambda: ext.attention_int4_kv(dual, **c), "q")):
             with pytest.raises(RuntimeError, match=name + " has a forward-mode tangent"):
                 call()
+
+
+def _class(**o):
+    from quant_pipeline.ops import Int4KVCache
+
+    return Int4KVCache(2, 16, 3, 128, 64, **o)
+
+
+@pytest.mark.parametrize("name", ["k_step", "v_step"])
+@pytest.mark.parametrize("step", [torch.ones(3, 3), torch.ones(3), torch.ones(2, 3, 2), torch.ones(3, 2).half(),
+                                  torch.ones((3, 2), dtype=torch.int32), 0.1], ids=str)
+def test_the_cache_class_refuses_bad_steps(name, step):
+    with pytest.raises(ValueError, match=name + " must be float32 \\[kv_heads, head_dim / group_size\\]"):
+        _class(**{name: step})
+
+
+def test_the_cache_class_takes_steps_as_constants_on_its_device():
+    param = torch.nn.Parameter(torch.arange(6.0).view(2, 3).t() + 1)  # not contiguous
+    cache = _class(k_step=param)
+    assert not cache.k_step.requires_grad and cache.k_step.is_contiguous() and cache.v_step is None
+    assert torch.equal(cache.k_step, param) and "k_step" in cache.state_dict() and not list(cache.parameters())
+    with torch.no_grad():
+        param.mul_(2)
+    assert torch.equal(cache.k_step * 2, param)
+    moved = _class(device=torch.device("meta"), k_step=param, v_step=torch.ones(3, 2))
+    assert moved.k_step.device.type == moved.v_step.device.type == moved.k_codes.device.type == "meta"
