@@ -1,7 +1,7 @@
 """Builds libw4a8.so (the C-ABI CUDA library) in-tree for sm_100a, and the
 small torch module _w4a8_torch.so beside it.
 
-Usage: python build_native.py [--force]
+Usage: python build_native.py [--force] [--library]   (--library: libw4a8.so alone)
 
 The library is self-contained (static CUDA runtime, no torch linkage); the
 Python module ``int4_int8_ext`` loads it with ctypes. _w4a8_torch.so holds the
@@ -63,18 +63,16 @@ def _build_binding(verbose: bool) -> None:
     os.replace(tmp, BINDING)
 
 
-def _stale() -> bool:
-    if not LIB.exists() or not BINDING.exists():
+def _stale(target: Path, deps) -> bool:
+    """Whether target is missing or older than what it is made from."""
+    if not target.exists():
         return True
-    lib_t = min(LIB.stat().st_mtime, BINDING.stat().st_mtime)
-    deps = [CSRC / s for s in SOURCES + DIM_SOURCES + HEADERS + [BINDING_SOURCE]] + [INCLUDE / "w4a8.h", Path(__file__)]
-    return any(d.stat().st_mtime > lib_t for d in deps if d.exists())
+    at = target.stat().st_mtime
+    return any(d.stat().st_mtime > at for d in [*deps, INCLUDE / "w4a8.h", Path(__file__)] if d.exists())
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compiles every CUDA source for sm_100a, links libw4a8.so, and builds the torch module."""
-    if not force and not _stale():
-        return LIB
+def _build_library(pool: ThreadPoolExecutor, verbose: bool) -> None:
+    """Compiles every CUDA source for sm_100a and links libw4a8.so."""
     objdir = HERE / "_build"
     objdir.mkdir(exist_ok=True)
     nvcc = _nvcc()
@@ -90,10 +88,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         subprocess.run(cmd, check=True)
         return str(obj)
 
-    with ThreadPoolExecutor(max_workers=max(1, min(len(units) + 1, os.cpu_count() or 1))) as pool:
-        binding = pool.submit(_build_binding, verbose)
-        objs = list(pool.map(compile_unit, units))
-        binding.result()
+    objs = list(pool.map(compile_unit, units))
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", str(tmp), *objs,
            "-Xcompiler", "-fPIC"]
@@ -101,9 +96,23 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, LIB)
+
+
+def build(force: bool = False, verbose: bool = False, torch_module: bool = True) -> Path:
+    """Builds libw4a8.so and, unless torch_module is False, the torch module beside it, where they are missing or older than
+    their sources. The library needs nvcc alone and is in place before a failure of the module is raised."""
+    library = force or _stale(LIB, [CSRC / s for s in SOURCES + DIM_SOURCES + HEADERS])
+    module = torch_module and (force or _stale(BINDING, [CSRC / BINDING_SOURCE]))
+    with ThreadPoolExecutor(max_workers=max(1, os.cpu_count() or 1)) as pool:
+        binding = pool.submit(_build_binding, verbose) if module else None
+        if library:
+            _build_library(pool, verbose)
+        if binding and binding.exception():
+            raise RuntimeError(f"libw4a8.so is built, the torch module {BINDING.name} is not: {binding.exception()}"
+                               ) from binding.exception()
     return LIB
 
 
 if __name__ == "__main__":
-    build(force="--force" in sys.argv, verbose=True)
+    build(force="--force" in sys.argv, verbose=True, torch_module="--library" not in sys.argv)
     print(LIB)
