@@ -44,6 +44,25 @@ def _nvcc() -> str:
     return str(cand) if cand.exists() else "nvcc"
 
 
+def _built_for() -> str:
+    """What a torch module fits: one torch and one Python."""
+    import torch
+
+    return f"torch {torch.__version__}, C++11 ABI {int(torch._C._GLIBCXX_USE_CXX11_ABI)}, {sysconfig.get_config_var('SOABI')}"
+
+
+def _note() -> Path:
+    """The file that says what the torch module was built for."""
+    return HERE / "_build" / (BINDING.stem + ".txt")
+
+
+def _fits() -> bool:
+    try:
+        return _note().read_text() == _built_for()
+    except (OSError, ImportError):
+        return False
+
+
 def _build_binding(verbose: bool) -> None:
     """Compiles _w4a8_torch.so against the installed torch."""
     import torch
@@ -61,6 +80,8 @@ def _build_binding(verbose: bool) -> None:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, BINDING)
+    _note().parent.mkdir(exist_ok=True)
+    _note().write_text(_built_for())
 
 
 def _stale(target: Path, deps) -> bool:
@@ -100,9 +121,9 @@ def _build_library(pool: ThreadPoolExecutor, verbose: bool) -> None:
 
 def build(force: bool = False, verbose: bool = False, torch_module: bool = True) -> Path:
     """Builds libw4a8.so and, unless torch_module is False, the torch module beside it, where they are missing or older than
-    their sources. The library needs nvcc alone and is in place before a failure of the module is raised."""
+    their sources, the module also where it was built for another torch or Python. The library needs nvcc alone and is in place before a failure of the module is raised."""
     library = force or _stale(LIB, [CSRC / s for s in SOURCES + DIM_SOURCES + HEADERS])
-    module = torch_module and (force or _stale(BINDING, [CSRC / BINDING_SOURCE]))
+    module = torch_module and (force or not _fits() or _stale(BINDING, [CSRC / BINDING_SOURCE]))
     with ThreadPoolExecutor(max_workers=max(1, os.cpu_count() or 1)) as pool:
         binding = pool.submit(_build_binding, verbose) if module else None
         if library:

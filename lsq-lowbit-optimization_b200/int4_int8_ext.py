@@ -556,7 +556,8 @@ def _load_binding():
     try:
         import _w4a8_torch as module
     except ImportError as e:
-        raise RuntimeError(f"torch module _w4a8_torch is not built. Run: python {_HERE / 'build_native.py'}") from e
+        raise RuntimeError(f"torch module _w4a8_torch is not built, or for another torch or Python ({e}). "
+                           f"Run: python {_HERE / 'build_native.py'}") from e
     module.set_library(*(ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in (
         "w4a8_kv_write_int4", "w4a8_kv_read_int4", "w4a8_attention_int4", "w4a8_attention_int4_workspace")))
     return module

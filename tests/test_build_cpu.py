@@ -51,3 +51,41 @@ def test_a_library_that_fails_is_reported_as_itself(fake):
     with pytest.raises(subprocess.CalledProcessError):
         build_native.build()
     assert not build_native.LIB.exists()
+
+
+def test_another_torch_or_python_rebuilds_the_module(fake, monkeypatch):
+    """The module fits one version of each; file times do not show that."""
+    build_native.build()
+    assert fake.built() == {"libw4a8.so", "_w4a8_torch.so"}
+    build_native.build()
+    assert fake.built() == set()
+    import torch
+
+    with monkeypatch.context() as m:
+        m.setattr(torch, "__version__", "99.0")
+        build_native.build()
+        assert fake.built() == {"_w4a8_torch.so"}
+        build_native.build()
+        assert fake.built() == set()
+    build_native.build()
+    assert fake.built() == {"_w4a8_torch.so"}
+    monkeypatch.setattr(build_native.sysconfig, "get_config_var", lambda name: "cpython-399")
+    build_native.build()
+    assert fake.built() == {"_w4a8_torch.so"}
+
+
+def test_a_module_that_does_not_fit_is_named_with_its_error(monkeypatch):
+    import sys
+
+    import int4_int8_ext as ext
+
+    class Finder:
+        def find_spec(self, name, path=None, target=None):
+            if name == "_w4a8_torch":
+                raise ImportError("undefined symbol: of another torch")
+
+    build_native.build()
+    monkeypatch.delitem(sys.modules, "_w4a8_torch", raising=False)
+    monkeypatch.setattr(sys, "meta_path", [Finder(), *sys.meta_path])
+    with pytest.raises(RuntimeError, match="undefined symbol: of another torch.*build_native.py"):
+        ext._load_binding()
