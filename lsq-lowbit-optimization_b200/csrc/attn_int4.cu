@@ -79,7 +79,8 @@ size_t workspace_of(const w4a8_kv_cache* c, int q_heads, const Plan& p) {
 }
 
 int check(const w4a8_kv_cache* c, int q_heads, int dtype, int max_q, int max_len, int window) {
-  if (!c || dtype < W4A8_F32 || dtype > W4A8_BF16 || c->heads < 1 || q_heads < 1 || q_heads % c->heads || max_q < 0 ||
+  if (!c || c->pages < 0 || c->page_size < 1 || c->batch < 0 || c->rows < 0 || c->table_cols < 0) return W4A8_ERR_ARG;
+  if (dtype < W4A8_F32 || dtype > W4A8_BF16 || c->heads < 1 || q_heads < 1 || q_heads % c->heads || max_q < 0 ||
       max_len < 0 || window < 0)
     return W4A8_ERR_ARG;
   if ((long long)c->table_cols * c->page_size > kKvMostTokens) return W4A8_ERR_UNSUPPORTED;
