@@ -231,10 +231,6 @@ template <typename T, int D, int G>
 __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const __grid_constant__ AttnParams p) {
   using Smem = PreSmem<D>;
   constexpr int kGroups = D / G, kChunks = D / 8;
-  // Masks as bits and a first guess of the reference make the first and last tile of a row cheaper. The code that
-  // the others then get is better with 64 channels (700 rows in a window of 1024: 70.0 -> 63.3 us) and worse with 128
-  // (8192 tokens: 657 -> 736 us), where the two query tiles fall into a less even step.
-  constexpr bool kQuickEdges = D <= 64;
   extern __shared__ uint8_t smem_raw[];
   __shared__ PreBars bars;
   __shared__ uint32_t tmem_base_s;
@@ -580,7 +576,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
       // passes m by more than kPreRaise (or at the first tile) m is raised, the output rescaled and the row done again, so
       // most tiles take one pass. They are held in registers until then, since
       // they go where the scores are. The next 32 columns are loaded while these are worked on.
-      if (kQuickEdges && j == 0) {  // nothing to go by yet: the largest of 32 columns that the rows of the warp see
+      // Nothing to go by at the first tile: the largest of 32 columns that the rows of the warp see. This and the masks
+      // as bits make the first and last tiles of a row cheaper: 6 chunks of 700 tokens in a window of 1024, 16 heads on 4
+      // of 64, 96 and 128 channels 77, 86 and 92 us without, 67, 74 and 81 with; 8192 tokens 591, 649 and 653 without, 592,
+      // 628 and 644 with.
+      if (j == 0) {
         const int c = min(max(__shfl_sync(0xffffffffu, from, 31), 0), kPreTile - 1) / 32;
         float y[32];
         tmem_ld32(s_addr + c * 32, y);
@@ -605,15 +605,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
           tmem_ld_wait32(y);
           if (c + 1 < kPreTile / 32) tmem_ld32(s_addr + (c + 1) * 32, x[(c + 1) & 1]);
           if (partial) {
-            if constexpr (kQuickEdges) {
-              const uint32_t seen = bits_between(from - c * 32, to - c * 32);
+            const uint32_t seen = bits_between(from - c * 32, to - c * 32);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) y[k] = seen >> k & 1 ? y[k] : kNegInf;
-            } else {
-#pragma unroll
-              for (int k = 0; k < 32; ++k)
-                if (c * 32 + k < from || c * 32 + k >= to) y[k] = kNegInf;
-            }
+            for (int k = 0; k < 32; ++k) y[k] = seen >> k & 1 ? y[k] : kNegInf;
           }
           float t[2] = {kNegInf, kNegInf};
 #pragma unroll
