@@ -20,7 +20,9 @@ struct Plan {
 // kMinChunk tokens, twice as many in a batch: below that its start and the join cost more than the tokens (1024 tokens
 // of one sequence: 7.4 us with 128, 8.0 with 256; 7 sequences of up to 2011: 16.4 and 13.1).
 constexpr int kWaves = 6, kMinChunk = kAttnWarps * kTile, kPreMinChunk = 4 * kPreTile;
-// From this many query rows a key head on, the tensor cores' tiles of 128 rows pay.
+// From this many query rows a key head on, the tensor cores' tiles of 128 rows pay. 8192 tokens, 8 heads of 128 channels, few-row
+// kernel and prompt kernel, us: 16 sequences of 48 rows 194 and 203, of 64 rows 250 and 200, of 128 rows 447 and 165. One
+// sequence alone, which few rows split finer: 64 rows 25 and 32, 96 rows 30 and 33, 128 rows 39 and 33. 64 channels alike.
 constexpr int kPrefillRows = 64;
 
 // Tensor maps of the codes, for boxes of 32 or 16 rows of a page; the rows of a box, or 0 where pages are

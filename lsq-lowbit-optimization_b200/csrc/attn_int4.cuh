@@ -666,14 +666,19 @@ __device__ __forceinline__ void attn_rows(const AttnParams& p, const KvSeq& seq,
     }
 
     // Weights 2^(s q_mul - m), q_mul > 0. m is raised only when some score passes it by more than 8:
-    // weights then stay below 2^8, and most tiles need no exchange between lanes and no rescaling.
+    // weights then stay below 2^8, and most tiles need no exchange between lanes and no rescaling. The product is rounded
+    // before m is taken off, as it was for m: of the largest score a fused one would leave what its rounding cut off.
     float top[NT][2];
     bool raise = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        top[nt][e] = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2])) * q_mul[nt][e];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) s[h][nt][e + 2 * k] = __fmul_rn(s[h][nt][e + 2 * k], q_mul[nt][e]);
+        top[nt][e] = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
         raise |= top[nt][e] > m[nt][e] + 8.0f;
       }
     if (__any_sync(0xffffffffu, raise)) {
@@ -702,7 +707,7 @@ __device__ __forceinline__ void attn_rows(const AttnParams& p, const KvSeq& seq,
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const float w = exp2_approx(fmaf(s[h][nt][e + 2 * k], q_mul[nt][e], -ref));
+            const float w = exp2_approx(__fsub_rn(s[h][nt][e + 2 * k], ref));
             s[h][nt][e + 2 * k] = w;
             l[nt][e] += w;
           }

@@ -15,7 +15,7 @@
 // All operands are float16. code * scale has at most 11 significant bits, so keys and values are exact
 // there for scales from 2^-17 to 2^12. Where the largest scale of a block's first tile is not within [2^-9, 2^8] they are
 // held divided by a power of two, one for the block's keys and one for its values. A block that meets a scale outside
-// of the range all the same (of a token that its rows see or not) says so, and kv_attn_redo_kernel takes its rows again with
+// of the range all the same (of a token that its rows see or not), or scores near 2^20, says so, and kv_attn_redo_kernel takes its rows again with
 // the arithmetic of few rows. Otherwise large values, hidden ones even, would set the unit that small ones are lost in. A
 // query is brought to a largest magnitude near 2^14 by a power of two. Weights are rounded to 11 bits, and to multiples of
 // 2^-31 of the row's largest: that is what a long tail of small weights beside one large is off by. Two float16 terms would need
@@ -59,6 +59,9 @@ constexpr int prefill_smem_bytes() {
 // Weights are 2^(score - m). m is set so that the largest is 2^kPreHigh, and raised when one would pass 2^kPreRaise: float16
 // goes up to 2^16, and what is small keeps bits down to 2^-24, which is 2^-31 of the largest or less.
 constexpr float kPreHigh = 7.0f, kPreRaise = 15.0f;
+// A fused multiply-add of a score keeps what the rounding of m cut off: up to 2^-4 for m below 2^20, beyond which rows are
+// handed over.
+constexpr float kPreMost = 0x1p20f;
 
 // Bits [from, to) of 32, either of them anywhere.
 __device__ __forceinline__ uint32_t bits_between(int from, int to) {
@@ -589,6 +592,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
 #pragma unroll
         for (int k = 0; k < 32; ++k) m = fmaxf(m, seen >> k & 1 ? y[k] : kNegInf);
         m = m * m32 - kPreHigh;
+        if (m != kNegInf && fabsf(m) > kPreMost) handover = 1;
       }
       uint32_t w[kPreTile / 2];
       float sum;
@@ -629,6 +633,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
         again = !again && __any_sync(0xffffffffu, top > m + kPreRaise);
         if (again) {
           const float next = fmaxf(m, top - kPreHigh);
+          if (next != kNegInf && fabsf(next) > kPreMost) handover = 1;
           const float c = next == kNegInf ? 1.0f : exp2_approx(m - next);
           m = next;
           l *= c;

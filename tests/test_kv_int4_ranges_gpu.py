@@ -134,3 +134,75 @@ def test_a_sink_with_small_values_and_a_long_tail(cuda, dtype, n):
     q, qt = typed(q, dtype)
     out, lse = ext.attention_int4_kv(qt.to(cuda), *s.tensors, *idx, scale=1.0 / 7, return_lse=True)
     kv_bounds.check(q, out, lse, s, dtype, 1.0 / 7, many=n > 32)
+
+
+def test_a_captured_call_decides_at_each_replay(cuda):
+    """A captured prompt over a cache whose scales are even, then far apart, then even again: as eager calls give it."""
+    s = Setup(59, [300], [150], 2, 64, 32, 16, cuda)
+    idx, _ = s.index()
+    _, qt = typed(s.g.standard_normal((150, 4, 64)), "bf16")
+    qt, even = qt.to(cuda), s.tensors[2].clone()
+    far = even.clone()
+    far[int(s.table[0][5])] *= 2.0 ** 40
+
+    def call():
+        return ext.attention_int4_kv(qt, *s.tensors, *idx, scale=0.05)
+
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for scales in (even, far, even, far):
+        s.tensors[2].copy_(scales)
+        graph.replay()
+        assert torch.equal(out, call()) and not out.isnan().any()
+    del graph
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_nan_values_beside_scales_far_apart(cuda, dtype):
+    """The rows that see the NaN give NaN in its group, the others what they gave without it."""
+    length, n, bad = 300, 150, 220
+    s = Setup(61, [length], [n], 1, 64, 32, 16, cuda)
+    k, v = (typed(s.g.standard_normal((length, 1, 64)), "bf16")[0] for _ in range(2))
+    v[180] *= 2.0 ** 40
+    _filled(s, k, v)
+    idx, _ = s.index()
+    _, qt = typed(s.g.standard_normal((n, 2, 64)), dtype)
+    run = lambda: ext.attention_int4_kv(qt.to(cuda), *s.tensors, *idx, scale=0.05, window=30)  # noqa: E731
+    want = run()
+    s.tensors[2][int(s.table[0][bad // 16]), 0, bad % 16, 1, 1] = float("nan")  # the second group's values
+    got = run()
+    pos = torch.arange(length - n, length, device=cuda)
+    sees = (pos >= bad) & (pos < bad + 30)
+    assert got[sees][..., 32:].isnan().all()
+    assert torch.equal(got[sees][..., :32], want[sees][..., :32]) and torch.equal(got[~sees], want[~sees])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n", [12, 150])
+@pytest.mark.parametrize("exp", [12, 20, 25, 30, 60])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("d", [64, 128])
+def test_scores_of_any_size(cuda, dtype, n, exp, sign, d):
+    """Scores from 7 2^exp to 56 2^exp, or their opposites, 2^-8 apart or more: the largest takes all of the weight, and the
+    output is its value. Keys of one channel, code 7 times a bfloat16 of each token's own: every product is exact."""
+    s = Setup(67 + exp, [300], [n], 1, d, 64, 16, cuda)
+    i = s.g.permutation(300)
+    k, v = np.zeros((300, 1, d)), s.g.standard_normal((300, 1, d))
+    k[:, 0, 0] = sign * 7 * (1 + i % 128 / 128) * 2.0 ** (i // 128 + exp - 3)
+    v = typed(v, "bf16")[0]
+    _filled(s, k, v)
+    idx, _ = s.index()
+    q = np.zeros((n, 2, d))
+    q[..., 0] = 8
+    out, lse = ext.attention_int4_kv(typed(q, dtype)[1].to(cuda), *s.tensors, *idx, scale=1.0, return_lse=True)
+    keys, values = s.cache.rows(0, s.table, 300)
+    scores = 8 * keys[:, 0, 0]
+    top = [np.argmax(scores[:p + 1]) for p in range(300 - n, 300)]
+    # One weight, off by its rounding and that of the sums; the output is rounded once.
+    half, weight = kv_bounds.HALF_STEP[dtype], 2.0 ** -20 + (2.0 ** -11 if n > 32 and dtype != "f32" else kv_bounds.WEIGHT[dtype])
+    for h in range(2):
+        err = np.abs(out[:, h].double().cpu().numpy() - values[top, 0])
+        assert np.all(err <= (half + weight + half * weight) * np.abs(values[top, 0]))
+        assert np.all(np.abs(lse[:, h].double().cpu().numpy() - scores[top]) <= 2.0 ** -21 * np.abs(scores[top]))
