@@ -665,8 +665,9 @@ __device__ __forceinline__ void attn_rows(const AttnParams& p, const KvSeq& seq,
       }
     }
 
-    // Weights 2^(s q_mul - m), q_mul > 0. m is raised only when some score passes it by more than 8:
-    // weights then stay below 2^8, and most tiles need no exchange between lanes and no rescaling. The product is rounded
+    // Weights 2^(s q_mul - m), q_mul > 0. m is raised only when some score passes it, and then to 8 above that score: most
+    // tiles need no exchange between lanes and no rescaling, and weights are at most 1, so that their sums with values
+    // near the largest number do not overflow before the mean of those does. The product is rounded
     // before m is taken off, as it was for m: of the largest score a fused one would leave what its rounding cut off.
     float top[NT][2];
     bool raise = false;
@@ -679,7 +680,7 @@ __device__ __forceinline__ void attn_rows(const AttnParams& p, const KvSeq& seq,
 #pragma unroll
           for (int k = 0; k < 2; ++k) s[h][nt][e + 2 * k] = __fmul_rn(s[h][nt][e + 2 * k], q_mul[nt][e]);
         top[nt][e] = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
-        raise |= top[nt][e] > m[nt][e] + 8.0f;
+        raise |= top[nt][e] > m[nt][e];
       }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -690,7 +691,7 @@ __device__ __forceinline__ void attn_rows(const AttnParams& p, const KvSeq& seq,
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          x = fmaxf(x, m[nt][e]);
+          x = x > m[nt][e] ? x + 8.0f : m[nt][e];
           const float c = x == kNegInf ? 1.0f : exp2_approx(m[nt][e] - x);
           m[nt][e] = x;
           l[nt][e] *= c;

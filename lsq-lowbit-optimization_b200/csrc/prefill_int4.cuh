@@ -58,7 +58,7 @@ constexpr int prefill_smem_bytes() {
 
 // Weights are 2^(score - m). m is set so that the largest is 2^kPreHigh, and raised when one would pass 2^kPreRaise: float16
 // goes up to 2^16, and what is small keeps bits down to 2^-24, which is 2^-31 of the largest or less.
-constexpr float kPreHigh = 7.0f, kPreRaise = 15.0f;
+constexpr float kPreHigh = 7.0f, kPreRaise = 15.0f, kPreLow = 0x1p-15f;
 // A fused multiply-add of a score keeps what the rounding of m cut off: up to 2^-4 for m below 2^20, beyond which rows are
 // handed over.
 constexpr float kPreMost = 0x1p20f;
@@ -667,7 +667,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
     if (!ok && lane == 0) atomicOr(v.err, kErrTimeoutEpilogue);
     tc_fence_after();
     const long long at = (long long)(seq.row0 + token) * p.q_heads + qh;
-    const float inv = p.splits > 1 ? units[1] : l == 0.0f ? 0.0f : __frcp_rn(l) * units[1];
+    // Partial results are for weights of at most 1: with larger ones the sums of values near the largest number overflow.
+    const float inv = units[1] * (p.splits > 1 ? kPreLow : l == 0.0f ? 0.0f : __frcp_rn(l));
 #pragma unroll
     for (int k = 0; k < D / 32; ++k) {
       float x[32];
@@ -702,7 +703,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_int4_kernel(const _
       }
     }
     if (mine) {
-      if (p.splits > 1) p.part_ml[at * p.splits + split] = make_float2(m, l);
+      if (p.splits > 1) p.part_ml[at * p.splits + split] = make_float2(m + kPreRaise, l * kPreLow);
       else if (p.lse) p.lse[at] = l == 0.0f ? kNegInf : (m + log2f(l)) * 0.69314718055994531f;
     }
     tc_fence_before();

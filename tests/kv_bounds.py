@@ -22,7 +22,8 @@ def attention_and_bound(q, setup, dtype, scale, causal=True, window=0, many=Fals
       to 8, and three sums are rounded to 24 bits;
     * the exponential and its argument, 2^-21 (1 + |score|);
     * its own rounding: WEIGHT, or with many rows 2^-11 and, relative to the row's largest weight, 2^-32 (the smallest float16 is
-      2^-24, and the reference weight 2^7). Weights below 2^-126 of the largest are zeros.
+      2^-24, and the reference weight 2^7). Weights below 2^-126 of the reference, which is 2^8 of the
+      largest weight at most, are zeros.
     Sums over the tokens take a step for 16 of them and each term, each off by 2^-22 of what was added up."""
     want, lse = kvo.attention(q, setup.cache, setup.table, setup.lens, setup.cu, scale, causal, window)
     off, lse_off = np.zeros(want.shape), np.zeros(lse.shape)
@@ -57,7 +58,7 @@ def attention_and_bound(q, setup, dtype, scale, causal=True, window=0, many=Fals
                 e = e + 2.0 ** -21 * (1 + np.abs(score))
                 lse_off[row, h] = (p * e).sum() + 2.0 ** -21 * (1 + abs(lse[row, h]))
                 e = e + (2.0 ** -11 if many else WEIGHT[dtype]) + (seen.sum() / 16 + 4) * terms * 2.0 ** -22
-                least = (2.0 ** -32 if many else 2.0 ** -126) * p.max()
+                least = (2.0 ** -32 if many else 2.0 ** -118) * p.max()
                 off[row, h] = (p * e + least) @ np.abs(vs) + (p * e).sum() * np.abs(want[row, h])
     return want, lse, off, lse_off
 

@@ -206,3 +206,35 @@ def test_scores_of_any_size(cuda, dtype, n, exp, sign, d):
         err = np.abs(out[:, h].double().cpu().numpy() - values[top, 0])
         assert np.all(err <= (half + weight + half * weight) * np.abs(values[top, 0]))
         assert np.all(np.abs(lse[:, h].double().cpu().numpy() - scores[top]) <= 2.0 ** -21 * np.abs(scores[top]))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n", [12, 150])
+@pytest.mark.parametrize("length,most", [(300, None), (3000, 3000)])  # the second is split
+def test_values_near_the_largest_numbers(cuda, dtype, n, length, most):
+    """Sums of up to 3000 weights of at most 1 with values below 2^116 do not overflow."""
+    s = Setup(71, [length], [n], 1, 64, 32, 16, cuda)
+    k, v = (s.g.standard_normal((length, 1, 64)) for _ in range(2))
+    v = np.clip(v, -3, 3) * 2.0 ** 114
+    k, v = (typed(x, "bf16")[0] for x in (k, v))
+    _filled(s, k, v)
+    q, (out, lse) = _run(cuda, s, dtype, 0.5, max_len=most)
+    assert out.isfinite().all()
+    kv_bounds.check(q, out, lse, s, dtype, 0.5, many=n > 32 and dtype != "f32")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n", [4, 150])
+def test_values_near_the_largest_numbers_behind_a_rising_score(cuda, dtype, n):
+    """A token whose score is 5 above those before it, and values of 2^123: no weight goes beyond the largest's 1."""
+    s = Setup(73, [160], [n], 1, 64, 32, 16, cuda)
+    k, v = np.zeros((160, 1, 64)), s.g.choice([-1.0, 1.0], (160, 1, 64)) * 2.0 ** 123
+    k[140, 0, 0] = 7
+    _filled(s, k, typed(v, "bf16")[0])
+    idx, _ = s.index()
+    q = np.zeros((n, 2, 64))
+    q[..., 0] = 5
+    q, qt = typed(q, dtype)
+    out, lse = ext.attention_int4_kv(qt.to(cuda), *s.tensors, *idx, scale=1 / 7, return_lse=True)
+    assert out.isfinite().all()
+    kv_bounds.check(q, out, lse, s, dtype, 1 / 7, many=n > 32 and dtype != "f32")
