@@ -11,9 +11,11 @@
 // fills 1/16 of a 128-row tensor-core tile, and unpacked operands would have to pass through
 // shared memory at four times the size of the codes. In registers they never leave the warp.
 //
-// Bound by instruction issue: about 600 instructions for 32 tokens of a head, a third of them the shifts and
-// logic that unpack. One sequence of 131072 tokens, 32 query heads on 8 of 128 channels, bfloat16:
-// 48 us, 3.0 TB/s. 64 sequences of up to 8192 tokens, 64 heads on 8: 108 us, 2.9 TB/s.
+// No unit is full: about 700 instructions for 32 tokens of a head, a quarter of them the shifts and logic that unpack, fill
+// 57 to 60% of the issue slots, 50% of the ALU's, 29% of the tensor cores', 39% of the memory's. A scheduler has 3.5
+// warps, which is what 128 registers a lane allow, and 1.2 of them can issue: their dependent instructions and the start
+// of a block bound it. One sequence of 131072 tokens, 32 query heads on 8 of 128 channels, bfloat16:
+// 47 us, 3.0 TB/s. 64 sequences of up to 8192 tokens, 64 heads on 8: 109 us, 2.8 TB/s.
 //
 // Codes. A 32-bit word of a row is eight channels; word & 0x000f000f is the pair (0, 4),
 // >> 8 the pair (2, 6). With the sign bit flipped a nibble is n = c + 8 >= 0.
@@ -22,17 +24,17 @@
 //    two, its pairs (1, 5) and (3, 7) are divided by 16, and the accumulators start at
 //    -8 2^-24 sum(q): sums of a group come out signed. They are multiplied by the key's scale in
 //    32 bits. (The tensor cores cut products off 25 bits below the largest of a step, and count a subnormal as 2^-14
-//    there: what a channel adds to a score is off by up to 2^-15 of the largest |q| times the key's scale.) For float32 queries 8 is subtracted from n first, and the query is two terms with sums of
-//    their own: the scaled query rounded to multiples of 8, whose sums are integers below 2^24 and so exact (the
-//    tensor cores cut off what lies below the largest product of a step), and what is left. Off by 2e-7 to 3e-7 for
-//    scores of standard deviation 4, 1e-6 to 2e-6 with two float16 roundings in one sum.
+//    there: what a channel adds to a score is off by up to 2^-15 of the largest |q| times the key's scale.)
+//    For float32 queries 8 is subtracted from n first, and the query is two terms with sums of their own: the scaled
+//    query rounded to multiples of 8, whose sums are integers below 2^24 and so exact in spite of that, and what is
+//    left. Off by 2e-7 to 3e-7 for scores of standard deviation 4, 1e-6 to 2e-6 with two float16 roundings in one sum.
 //  * Values: as bfloat16 bits, 0x4300 | n is 128 + n, and 136 is subtracted (exact). Here the
 //    sums run over thousands of tokens and would cancel 136 sum(p) to its last bits.
 // Weights times the value's scale are bfloat16 terms, whose range is that of the scales: two, which keep 15 bits, and
 // for float32 queries three (24 bits), with a product each. The two come from two terms of the weight by three bfloat16
-// multiply-adds, since what the first product leaves is exact in bfloat16. With one term only a call takes 44.5 us in place
-// of 48.3 (131072 tokens) and 97 in place of 108 (64 sequences), but its rounding adds as much to the error as that of a bfloat16
-// output: 2.3e-3 against 1.7e-3 from the formula in 64 bits.
+// multiply-adds, since what the first product leaves is exact in bfloat16. With one term a call took 44 us in place of
+// 47 (131072 tokens) and 97 in place of 108 (64 sequences), but its rounding adds as much to the error as that of a
+// bfloat16 output: 2.3e-3 against 1.7e-3 from the formula in 64 bits.
 #pragma once
 
 #include "kv_cache.cuh"
@@ -335,7 +337,7 @@ constexpr int attn_smem_bytes() {
 }
 
 // Blocks an SM is to hold: what the registers of a lane allow (sums, the query, scores), and the stages.
-// 131072 tokens, 128 channels, bfloat16: 43 us with 4, 52 with 3, 50 with 5.
+// 131072 tokens, 128 channels, bfloat16, with one term of a weight: 43 us with 4, 52 with 3, 50 with 5.
 constexpr int attn_blocks_sm(int d, int nt, bool f32) {
   return nt == 1 && d <= 128 && !f32 ? 4 : nt == 1 && d <= 128 ? 3 : 2;
 }

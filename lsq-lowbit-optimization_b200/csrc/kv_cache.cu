@@ -5,7 +5,7 @@
 // computed once. A block finds its rows' places in the cache once (sequence, length, page: a chain
 // of three loads), behind the first loads of the rows. A warp's accesses are whole lines on the float side, and a
 // group's largest magnitude is a butterfly over G / 8 neighbouring lanes. 8 heads of 128 channels, bfloat16: 16384
-// tokens are written in 24 us (3.5 TB/s, 147 instructions for eight channels), 65536 read in 61 us (5.6 TB/s).
+// tokens are written in 24 us (3.5 TB/s, 145 instructions for eight channels), 65536 read in 59 us (5.8 TB/s).
 #include <algorithm>
 #include <cstring>
 #include <type_traits>
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_int4_kernel(const __grid_con
 // A block has columns side by side and rows below each other for its threads. Its rows are shared out so that
 // all blocks run at once, four an SM, if that takes at most eight times kUnroll loads of a thread (5 prompts of 1237
 // rows of 12 heads of 96, float32, written and read: 15.3 -> 13.0 us; 16384 tokens of 8 heads of 128, bfloat16: 47 ->
-// 45); beyond that four times kUnroll are best (65536 tokens read: 60.7 us, 62.2 with eight).
+// 45); beyond that four times kUnroll are best (65536 tokens read, by read-only loads then: 60.7 us, 62.2 with eight).
 template <typename P>
 int launch_rows(void (*kern)(P), P p, cudaStream_t st) {
   const KvView& v = p.view;

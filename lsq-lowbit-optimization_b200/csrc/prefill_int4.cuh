@@ -8,9 +8,10 @@
 // made the other's products run. A 128-token tile of codes is read once for 256 rows, and unpacked operands
 // live in shared memory only.
 //
-// Bound by the chain of each tile: scores, weights, their hand-over, products; 4.8 k cycles for 128 tokens of 256
+// Bound by the chain of each tile: scores, weights, their hand-over, products; 4.7 k cycles for 128 tokens of 256
 // rows of 128 channels, in which the exponentials alone take 2 k and the products 1.5 k. 8192 tokens, causal, 32
-// query heads on 8 of 128 channels, bfloat16: 668 us, 823 TFLOP/s (half of the rate of a plain bfloat16 matrix product).
+// query heads on 8 of 128 channels, bfloat16: 650 us, 846 TFLOP/s in short runs (half of the rate of a plain bfloat16
+// matrix product), 680 us once the power limit lowers the clock.
 //
 // All operands are float16. code * scale has at most 11 significant bits, so keys and values are exact
 // there for scales from 2^-17 to 2^12. Where the largest scale of a block's first tile is not within [2^-9, 2^8] they are
