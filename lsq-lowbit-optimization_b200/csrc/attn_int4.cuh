@@ -27,7 +27,7 @@
 //    there: what a channel adds to a score is off by up to 2^-15 of the largest |q| times the key's scale.)
 //    For float32 queries 8 is subtracted from n first, and the query is two terms with sums of their own: the scaled
 //    query rounded to multiples of 8, whose sums are integers below 2^24 and so exact in spite of that, and what is
-//    left. Off by 2e-7 to 3e-7 for scores of standard deviation 4, 1e-6 to 2e-6 with two float16 roundings in one sum.
+//    left. Off by 3e-7 for scores of standard deviation 4, 1e-6 to 2e-6 with two float16 roundings in one sum.
 //  * Values: as bfloat16 bits, 0x4300 | n is 128 + n, and 136 is subtracted (exact). Here the
 //    sums run over thousands of tokens and would cancel 136 sum(p) to its last bits.
 // Weights times the value's scale are bfloat16 terms, whose range is that of the scales: two, which keep 15 bits, and
@@ -65,7 +65,7 @@ struct AttnParams {
   int row_tiles;            // tiles of 8 NT query rows of a key head
   int splits, chunk;        // blocks a sequence, tokens a block
   float* part_o;            // [rows * q_heads][splits][D]
-  float2* part_ml;          // [rows * q_heads][splits]: largest score (log2), sum of weights
+  float2* part_ml;          // [rows * q_heads][splits]: what scores are taken relative to (log2), sum of weights
   int* handover;            // many rows: for each block, whether its rows are left to kv_attn_redo_kernel
 };
 

@@ -16,11 +16,13 @@
 // All operands are float16. code * scale has at most 11 significant bits, so keys and values are exact
 // there for scales from 2^-17 to 2^12. Where the largest scale of a block's first tile is not within [2^-9, 2^8] they are
 // held divided by a power of two, one for the block's keys and one for its values. A block that meets a scale outside
-// of the range all the same (of a token that its rows see or not), or scores near 2^20, says so, and kv_attn_redo_kernel takes its rows again with
-// the arithmetic of few rows. Otherwise large values, hidden ones even, would set the unit that small ones are lost in. A
-// query is brought to a largest magnitude near 2^14 by a power of two. Weights are rounded to 11 bits, and to multiples of
-// 2^-31 of the row's largest: that is what a long tail of small weights beside one large is off by. Two float16 terms would need
-// twice the products and registers that a row does not have; error of float16 outputs 2.7e-4, of their own rounding 2.0e-4.
+// of the range all the same (of a token that its rows see or not), or scores near 2^20, says so, and
+// kv_attn_redo_kernel takes its rows again with the arithmetic of few rows. Otherwise large values, hidden ones even,
+// would set the unit that small ones are lost in. A query is brought to a largest magnitude near 2^14 by a power of two.
+//
+// Weights are rounded to 11 bits, and to multiples of 2^-31 of the row's largest: that is what a long tail of small
+// weights beside one large is off by. Two float16 terms would need twice the products and registers that a row does
+// not have; error of float16 outputs 2.7e-4, of their own rounding 2.0e-4.
 //
 // TMEM (512 columns): S of tile 0 and 1 at 0 and 128, their weights over them; O at 256 and 384.
 //

@@ -60,3 +60,24 @@ def test_many_rows_in_few_row_tiles_joined_from_splits(cuda, dtype):
     out, lse = ext.attention_int4_kv(qt.to(cuda), *s.tensors, *idx, cu_q=cu, max_q=5, max_len=max(lens), scale=0.02,
                                      return_lse=True)
     kv_bounds.check(q, out, lse, s, dtype, 0.02)
+
+
+@pytest.mark.parametrize("d,group", [(64, 64), (128, 32), (256, 128)])
+def test_float32_scores_are_sums_without_rounding_but_the_querys_own(cuda, d, group):
+    """One token a sequence: the logarithm is its score. In units of 2^-14 to 2^-13 of the largest |q|, times the scales, a channel is
+    off by its query's second term, rounded by 2^-10 at most, times a code of up to 8. Such errors are independent: the root
+    of their mean square is sqrt(d) 8 2^-10 / sqrt(3) = 0.07 for 256 channels. Scores of up to 2^19 units are rounded four times
+    to 24 bits, each off by 2^-6 / sqrt(3) at most: 0.02 together. (Products cut off at 1/4 would show as sqrt(d) / 14, 0.6 and more.)"""
+    batch = 512
+    s = Setup(37, [1] * batch, [1] * batch, 1, d, group, 16, cuda)
+    idx, _ = s.index()
+    q, qt = typed(s.g.standard_normal((batch, 8, d)), "f32")
+    scale = d ** -0.5
+    _, lse = ext.attention_int4_kv(qt.to(cuda), *s.tensors, *idx, scale=scale, return_lse=True)
+    keys = np.stack([s.cache.rows(b, s.table, 1)[0][0, 0] for b in range(batch)])
+    want = np.einsum("bhd,bd->bh", q, keys) * scale
+    steps = s.cache.scales[0][s.table[:, 0], 0, 0].max(-1)
+    unit = np.exp2(np.frexp(np.abs(q).max(-1))[1] - 14.0) * steps[:, None] * scale
+    assert np.abs(want / unit).max() < 2 ** 19
+    off = (lse.double().cpu().numpy() - want) / unit
+    assert np.sqrt((off ** 2).mean()) <= 0.1 and np.abs(off).max() <= 8 * d * 2.0 ** -10 + 4 * 2.0 ** -6
